@@ -1,0 +1,87 @@
+/* ridgefill_serve.h -- the serving rows: what a program runs over the caches that the fill rows write. Attention of a
+ * prompt's exact rows, attention of one new token over the paged K/V cache, and the DeltaNet layers' step for one new
+ * token. No counterpart in the reference: its engine answers with its own attention and recurrent kernels, whose
+ * source is not part of the checkout; here they read what ridgefill_attn_kv_fill and ridgefill_gdn_fill wrote.
+ *
+ * The rows are described by the plugin's own types (RadOpSchema, RadKernelInfo) and called like every row: RadArgs
+ * with operands in schema order, a cudaStream_t, a workspace where the row's scratch hook asks for one. They stand in
+ * a table of their own beside the plugin's, whose op list is the reference plugin's and its fill ops': a program that
+ * serves reads both (ridgefill_serve_count / _at).
+ *
+ * Every row launches on the stream it is given, allocates nothing and never synchronises; calls may be captured into
+ * a graph. Values in device memory (lengths, page and slot numbers) are read where the kernel runs, with a fail-safe:
+ * cu_seqlens and lengths are clamped into their operands, a page or slot outside its pool is not read or written.
+ * A call's workspace is its own until the call has run: calls that may overlap on the GPU need one each.
+ */
+#ifndef RIDGEFILL_SERVE_H
+#define RIDGEFILL_SERVE_H
+
+#include "ridgefill.h"
+
+/* ridgefill_attn_decode: operand positions. */
+enum { AD_Q = 0, AD_CACHE, AD_TABLE, AD_LENS, AD_O };
+/* ridgefill_gdn_step */
+enum { GS_Q = 0, GS_K, GS_V, GS_G, GS_BETA, GS_STATE, GS_STATE_IDX, GS_OUT_IDX, GS_O };
+
+/* ridgefill_attn_decode: one new token a sequence over the paged cache. Sequence i's key j (0 <= j < lens[i]) lies in
+ * slot table[i, j / page] * page + j % page of cache [2, slots, Hkv, D]; query head h reads kv head h / (Hq / Hkv):
+ *     o[i, h] = sum_j p_j cache[1, slot_j] / sum_j p_j,   p_j = exp(scale q[i, h] . cache[0, slot_j])
+ * over the keys whose slot lies in [0, slots); zeros when there is none. The products q . k are exact bf16 products
+ * summed in f32; p is held in f32 for the sum and as a bf16 pair (its rounding and the rest) for the product with v. */
+typedef struct RidgeFillAttnDecode {
+    const uint16_t* q;       int64_t q_row, q_head;              /* [B, Hq, D] */
+    const uint16_t* cache;   int64_t c_kv, c_slot, c_head, n_slots;   /* [2, slots, Hkv, D] */
+    const int32_t*  table;   int64_t t_row, n_pages;             /* [B, n_pages] */
+    const int32_t*  lens;                                        /* [B] */
+    uint16_t*       o;       int64_t o_row, o_head;              /* [B, Hq, D] */
+    int64_t         B, n_head, n_head_kv, head_dim, page;
+    float           scale;
+} RidgeFillAttnDecode;
+
+/* ridgefill_gdn_step: the gated delta rule for one new token a row (ridgefill_gdn_fill's rule on one-row sequences).
+ * Per row i and v-head h (k-head h / (Hv / Hk)), S the state in slot idx[i]:
+ *     S <- exp(g[i, h]) S;  S <- S + beta[i, h] (v - S k) k^T;  o[i, h] = scale S q
+ * the new S written to slot out_idx[i] (idx[i] without out_idx), in f32 throughout, o rounded once to bf16. A row is
+ * skipped -- no state and no o written -- when one of its slots lies outside the pool, or when the slot it would
+ * write is named by another row (written or read by it): rows that share a slot have no order among themselves. */
+typedef struct RidgeFillGdnStep {
+    const uint16_t* q;       int64_t q_row, q_head;              /* [B, Hk, dk] */
+    const uint16_t* k;       int64_t k_row, k_head;              /* [B, Hk, dk] */
+    const uint16_t* v;       int64_t v_row, v_head;              /* [B, Hv, dv] */
+    const float*    g;       int64_t g_row;                      /* [B, Hv] */
+    const float*    beta;    int64_t b_row;
+    float*          state;   int64_t st_slot, st_head, n_states; /* [slots, Hv, dv, dk] */
+    const int32_t*  idx;     int64_t idx_pitch;
+    const int32_t*  out_idx; int64_t out_pitch;                  /* null: in place */
+    uint16_t*       o;       int64_t o_row, o_head;              /* [B, Hv, dv] */
+    int64_t         B, n_head_k, n_head_v, dk, dv;
+    float           scale;
+} RidgeFillGdnStep;
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* The serving rows' schemas and rows (null past the end). */
+int                  ridgefill_serve_schema_count(void);
+const RadOpSchema*   ridgefill_serve_schema_at(int i);
+int                  ridgefill_serve_count(void);
+const RadKernelInfo* ridgefill_serve_at(int i);
+
+/* Parses: RAD_OK or a named refusal (null operands and missing parameters RAD_E_INVAL, types RAD_E_DTYPE, ranks and
+ * extents RAD_E_SHAPE, strides and alignment RAD_E_STRIDE, geometry no kernel serves RAD_E_UNSUPPORTED). */
+int ridgefill_attn_decode_parse(const RadArgs* a, RidgeFillAttnDecode* out);
+int ridgefill_gdn_step_parse(const RadArgs* a, RidgeFillGdnStep* out);
+
+/* The device rows: async launches on `s` (a cudaStream_t); no allocation, no synchronisation. */
+int ridgefill_attn_decode_device(const RadArgs* a, RadStream s);
+int ridgefill_gdn_step_device(const RadArgs* a, RadStream s);
+
+/* Scratch hooks: device bytes the call needs in RadArgs::scratch (16-byte aligned); 0: none. */
+int64_t ridgefill_attn_decode_scratch(const RadArgs* a);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* RIDGEFILL_SERVE_H */

@@ -1,0 +1,510 @@
+/* attn_decode.cu -- ridgefill_attn_decode: attention of one new token a sequence over the paged K/V cache, on B200
+ * (ridgefill_serve.h holds the formula; ridgefill_attn_kv_fill writes the cache).
+ *
+ * HBM-bound: the keys and values of every sequence are read once (1 KiB a key and kv head), and all of a kv head's
+ * query heads are served from that read. The arithmetic (4 D flops a key and query head) goes through mma.sync, far
+ * below its rate. What decides the time is how evenly the bytes spread over the SMs and how many are in flight.
+ *
+ * Work. A unit is 64 keys of one item (a sequence's kv head and up to 16 of its query heads). The units of all items
+ * in order -- sequence, head, position -- are cut into equal spans, one a CTA, whatever the lengths: a long sequence
+ * spreads over many CTAs, short ones share one. The lengths are device memory, so every CTA finds its span from
+ * kv_lens itself. A span that covers a whole item writes its output; the at most two items a span cuts leave a partial
+ * result (unnormalised sum, running maximum, sum of weights) in the CTA's two scratch slots, and the join kernel, whose
+ * launch overlaps this one's run, adds the pieces of each item.
+ *
+ * Inside a CTA four warps take 16-key blocks in turn, each with running softmax statistics of its own, and meet at the
+ * piece's end. A warp streams its blocks through its own ring in shared memory by 16-byte asynchronous copies that each
+ * lane issues and reads back itself: no barrier, no bank conflict, and two to three 8 KiB halves in flight a warp (128 KiB
+ * a SM; the 44 bytes a nanosecond of a SM's share of HBM at about a microsecond's latency need 44 KiB). The products are
+ * taken transposed, S^T = K Q^T and O^T = V^T P^T, so that the up to 8 query heads sharing a kv head fill the n of
+ * m16n8k16 exactly:
+ *   lane (r = lane / 4, c = lane % 4) holds keys r and r + 8, elements 32 j + 8 c .. + 7 of K: the A operand up to an
+ *   order of the contracted elements that Q shares; P^T goes from accumulators to the B operand by movmatrix; V^T's A
+ *   operand pairs the keys 2c, 2c+1, 2c+8, 2c+9 of elements 64 j + 8 r .. + 7 by byte permutes, and the accumulators
+ *   come out as eight consecutive elements a lane and head.
+ */
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "mma.cuh"
+#include "ridgefill_serve.h"
+
+namespace {
+
+constexpr int D = 256;
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kBlock = 16;                          /* keys a warp takes at a time */
+constexpr int kUnit = kWarps * kBlock;              /* keys of a unit */
+constexpr int kHalfBytes = kBlock * D * 2;          /* a block's keys, or its values */
+constexpr int kRing = 3;                            /* halves of a warp's ring */
+constexpr int kSmem = kWarps * kRing * kHalfBytes;
+constexpr int kCtasPerSm = 2;
+constexpr float kGrow = 8.0f;                       /* a maximum may be exceeded by 2^8 before the sums are rescaled */
+constexpr float kNone = -INFINITY;
+
+/* Query heads a CTA serves at once: 8 NT (NT the n-tiles of 8 heads). */
+template <int NT>
+struct Partial {                                    /* one piece's result */
+    float o[8 * NT][D];
+    float m[8 * NT], l[8 * NT];                     /* maximum (log2 units) and sum of 2^(s - m) */
+};
+
+struct Plan {
+    RidgeFillAttnDecode g;
+    int group, chunks;      /* query heads a kv head; items a kv head (group / heads of an item, rounded up) */
+    int ctas;               /* CTAs of the split kernel */
+    void* partials;         /* [ctas][2] Partial; null: one CTA an item, nothing to join */
+    float scale_log2;
+};
+
+__device__ __forceinline__ int64_t length_of(const RidgeFillAttnDecode& g, int64_t b) {
+    const int64_t most = g.n_pages * g.page, n = g.lens[b];
+    return n < 0 ? 0 : (n > most ? most : n);
+}
+__device__ __forceinline__ int64_t units_of(const RidgeFillAttnDecode& g, int64_t b) { return (length_of(g, b) + kUnit - 1) / kUnit; }
+
+/* Units of sequences [0, n) of one kv head and chunk; the whole warp. */
+__device__ __forceinline__ int64_t units_before(const RidgeFillAttnDecode& g, int64_t n, int lane) {
+    int64_t sum = 0;
+    for (int64_t b = lane; b < n; b += 32) sum += units_of(g, b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+    return *(const uint32_t*)&p;
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+
+/* One warp's walk over the 16-key blocks of a piece. */
+struct Blocks {
+    const uint16_t* keys;      /* cache plane 0 at the item's kv head */
+    int64_t len;               /* the sequence's keys */
+    const int32_t* table;      /* its pages */
+};
+
+/* The slot of key `j` (-1: past the sequence, or outside the pool), by the lane that owns it. */
+__device__ __forceinline__ int slot_of(const RidgeFillAttnDecode& g, const Blocks& w, int64_t j) {
+    if (j >= w.len) return -1;
+    const int page = (int)g.page, n = (int)j / page;
+    const int64_t slot = (int64_t)w.table[n] * page + ((int)j - n * page);
+    return slot >= 0 && slot < g.n_slots ? (int)slot : -1;
+}
+
+/* Lane's copies of one half (K when !values, else V) of the block whose slots the lanes 0..15 hold in `slots`. */
+__device__ __forceinline__ void fetch(const RidgeFillAttnDecode& g, const Blocks& w, int slots, bool values, uint8_t* half, int lane) {
+    const int r = lane >> 2, c = lane & 3;
+    if (!values) {
+        const int s0 = __shfl_sync(0xffffffffu, slots, r), s1 = __shfl_sync(0xffffffffu, slots, r + 8);
+        const uint16_t* p0 = w.keys + (int64_t)max(s0, 0) * g.c_slot + 8 * c;
+        const uint16_t* p1 = w.keys + (int64_t)max(s1, 0) * g.c_slot + 8 * c;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+            rf::cp_async16(half + (2 * j) * 512 + lane * 16, p0 + 32 * j, s0 >= 0 ? 16 : 0);
+            rf::cp_async16(half + (2 * j + 1) * 512 + lane * 16, p1 + 32 * j, s1 >= 0 ? 16 : 0);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = __shfl_sync(0xffffffffu, slots, 2 * c + (i & 1) + (i >> 1) * 8);
+            const uint16_t* p = w.keys + g.c_kv + (int64_t)max(s, 0) * g.c_slot + 8 * r;
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j) rf::cp_async16(half + (4 * j + i) * 512 + lane * 16, p + 64 * j, s >= 0 ? 16 : 0);
+        }
+    }
+    rf::cp_async_commit();
+}
+
+/* A piece's keys [from, to) of item (b, kv head, first query head h0, heads), by the whole CTA; its result to the
+ * output (`out`) or to `part`. */
+template <int NT>
+__device__ __forceinline__ void run_piece(const Plan& p, uint8_t* smem, int64_t b, int64_t hkv, int h0, int heads, int64_t from,
+                                          int64_t to, Partial<NT>* part) {
+    const RidgeFillAttnDecode& g = p.g;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
+    uint8_t* ring = smem + warp * kRing * kHalfBytes;
+    const Blocks w = { g.cache + hkv * g.c_head, length_of(g, b), g.table + b * g.t_row };
+    const int64_t first = from + warp * kBlock;
+    const int n = first < to ? (int)((to - first + kUnit - 1) / kUnit) : 0;   /* this warp's blocks */
+
+    float o[NT][D / 16][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        m[t][0] = m[t][1] = kNone;
+        l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
+    }
+    /* Q's operand: lane's elements 32 j + 8 c .. + 7 of query heads r (+ 8 a tile); heads past the item's are zero */
+    uint4 q[NT][D / 32];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int h = 8 * t + r;
+        const uint16_t* src = g.q + b * g.q_row + (hkv * p.group + h0 + h) * g.q_head + 8 * c;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) q[t][j] = h < heads ? *(const uint4*)(src + 32 * j) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    /* halves 2 i (keys) and 2 i + 1 (values) of block i go through slot (2 i) % kRing, ... of the ring, kRing - 1 ahead */
+    int cur = -1, next = -1;   /* lanes 0..15: the slots of blocks i and i + 1 */
+    if (n > 0) {
+        cur = slot_of(g, w, first + (lane & 15));
+        next = n > 1 ? slot_of(g, w, first + kUnit + (lane & 15)) : -1;
+        fetch(g, w, cur, false, ring, lane);
+        fetch(g, w, cur, true, ring + kHalfBytes, lane);
+    }
+    int at = 0;   /* ring slot of the current half */
+    for (int i = 0; i < n; ++i) {
+        const int after = i + 2 < n ? slot_of(g, w, first + (int64_t)(i + 2) * kUnit + (lane & 15)) : -1;
+        /* scores of the block's 16 keys */
+        int free_slot = at + 2 >= kRing ? at + 2 - kRing : at + 2;
+        if (i + 1 < n) fetch(g, w, next, false, ring + free_slot * kHalfBytes, lane);
+        else rf::cp_async_commit();
+        rf::cp_async_wait<2>();
+        float s[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+        const uint8_t* kh = ring + at * kHalfBytes + lane * 16;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+            const uint4 k0 = *(const uint4*)(kh + (2 * j) * 512), k1 = *(const uint4*)(kh + (2 * j + 1) * 512);
+            const uint32_t a0[4] = { k0.x, k1.x, k0.y, k1.y }, a1[4] = { k0.z, k1.z, k0.w, k1.w };
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                rf::mma_bf16(s[t], a0, q[t][j].x, q[t][j].y);
+                rf::mma_bf16(s[t], a1, q[t][j].z, q[t][j].w);
+            }
+        }
+        at = at + 1 == kRing ? 0 : at + 1;
+        const bool live0 = __shfl_sync(0xffffffffu, cur, r) >= 0, live1 = __shfl_sync(0xffffffffu, cur, r + 8) >= 0;
+        uint32_t phi[NT][2], plo[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            /* heads 2 c and 2 c + 1 of the tile: keys r and r + 8 here, the others across the lanes of one c */
+            float x[4], top[2];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = (e < 2 ? live0 : live1) ? s[t][e] * p.scale_log2 : kNone;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                top[e] = fmaxf(x[e], x[e + 2]);
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], d));
+            }
+            /* the maximum is followed only when it has grown by more than kGrow: until then the weights stay below 2^8 */
+            const bool grow = top[0] > m[t][0] + kGrow || top[1] > m[t][1] + kGrow;
+            if (__any_sync(0xffffffffu, grow)) {
+                float f[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float up = fmaxf(m[t][e], top[e]);
+                    f[e] = m[t][e] == kNone ? 0.f : exp2_approx(m[t][e] - up);
+                    m[t][e] = up;
+                    l[t][e] *= f[e];
+                }
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                    o[t][d][0] *= f[0];
+                    o[t][d][1] *= f[1];
+                    o[t][d][2] *= f[0];
+                    o[t][d][3] *= f[1];
+                }
+            }
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                y[e] = x[e] == kNone ? 0.f : exp2_approx(x[e] - m[t][e & 1]);
+                l[t][e & 1] += y[e];
+            }
+            /* p as its bf16 rounding and the bf16 rounding of the rest: 16 bits of it reach the product with v */
+            const uint32_t h01 = pack(y[0], y[1]), h23 = pack(y[2], y[3]);
+            phi[t][0] = transpose8x8(h01);
+            phi[t][1] = transpose8x8(h23);
+            plo[t][0] = transpose8x8(pack(y[0] - __uint_as_float(h01 << 16), y[1] - __uint_as_float(h01 & 0xffff0000u)));
+            plo[t][1] = transpose8x8(pack(y[2] - __uint_as_float(h23 << 16), y[3] - __uint_as_float(h23 & 0xffff0000u)));
+        }
+        /* O^T += V^T P^T */
+        free_slot = at + 2 >= kRing ? at + 2 - kRing : at + 2;
+        if (i + 1 < n) fetch(g, w, next, true, ring + free_slot * kHalfBytes, lane);
+        else rf::cp_async_commit();
+        rf::cp_async_wait<2>();
+        const uint8_t* vh = ring + at * kHalfBytes + lane * 16;
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+            uint4 v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = *(const uint4*)(vh + (4 * j + e) * 512);
+            const uint32_t* v0 = &v[0].x;
+            const uint32_t* v1 = &v[1].x;
+            const uint32_t* v2 = &v[2].x;
+            const uint32_t* v3 = &v[3].x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t a[4] = { __byte_perm(v0[e], v1[e], 0x5410), __byte_perm(v0[e], v1[e], 0x7632),
+                                        __byte_perm(v2[e], v3[e], 0x5410), __byte_perm(v2[e], v3[e], 0x7632) };
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    rf::mma_bf16(o[t][4 * j + e], a, phi[t][0], phi[t][1]);
+                    rf::mma_bf16(o[t][4 * j + e], a, plo[t][0], plo[t][1]);
+                }
+            }
+        }
+        at = at + 1 == kRing ? 0 : at + 1;
+        cur = next;
+        next = after;
+    }
+    rf::cp_async_wait<0>();
+
+    /* the warps' results meet in shared memory (over the rings, once every warp is done with its own) */
+    Partial<NT>* mine = (Partial<NT>*)smem;
+    static_assert(kWarps * sizeof(Partial<NT>) <= (size_t)kSmem, "the warps' results fit over the rings");
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float sum = l[t][e];
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            const int h = 8 * t + 2 * c + e;
+            if (r == 0) {
+                mine[warp].m[h] = m[t][e];
+                mine[warp].l[h] = sum;
+            }
+            /* elements 64 j + 8 r .. + 7 of head h: tiles 4 j .. 4 j + 3, two elements each */
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf)
+                    *(float4*)&mine[warp].o[h][64 * j + 8 * r + 4 * hf] =
+                        make_float4(o[t][4 * j + 2 * hf][e], o[t][4 * j + 2 * hf][2 + e], o[t][4 * j + 2 * hf + 1][e],
+                                    o[t][4 * j + 2 * hf + 1][2 + e]);
+        }
+    __syncthreads();
+    for (int x = threadIdx.x; x < heads * (D / 4); x += kThreads) {
+        const int h = x / (D / 4), d = (x % (D / 4)) * 4;
+        float top = kNone, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) top = fmaxf(top, mine[i].m[h]);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+            const float f = mine[i].m[h] == kNone ? 0.f : exp2_approx(mine[i].m[h] - top);
+            const float4 v = *(const float4*)&mine[i].o[h][d];
+            sum = fmaf(f, mine[i].l[h], sum);
+            acc.x = fmaf(f, v.x, acc.x);
+            acc.y = fmaf(f, v.y, acc.y);
+            acc.z = fmaf(f, v.z, acc.z);
+            acc.w = fmaf(f, v.w, acc.w);
+        }
+        if (part) {
+            *(float4*)&part->o[h][d] = acc;
+            if (d == 0) {
+                part->m[h] = top;
+                part->l[h] = sum;
+            }
+        } else {
+            const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);   /* no key: zeros; a NaN stays one */
+            *(uint2*)(g.o + b * g.o_row + (hkv * p.group + h0 + h) * g.o_head + d) =
+                make_uint2(pack(acc.x * inv, acc.y * inv), pack(acc.z * inv, acc.w * inv));
+        }
+    }
+    __syncthreads();   /* the results are read before the next piece's copies land */
+}
+
+/* CTA i's first unit of `total`; the CTA whose span holds unit u. */
+__device__ __forceinline__ int64_t span_of(const Plan& p, int64_t total, int64_t i) { return i * total / p.ctas; }
+__device__ __forceinline__ int64_t owner_of(const Plan& p, int64_t total, int64_t u) { return ((u + 1) * p.ctas - 1) / total; }
+
+template <int NT>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Plan p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    const RidgeFillAttnDecode& g = p.g;
+    const int lane = threadIdx.x & 31;
+    const int per_kv = p.chunks, items = (int)g.n_head_kv * per_kv;   /* items of a sequence */
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   /* the join may take its place on the SMs */
+    if (!p.partials) {   /* one CTA an item */
+        const int64_t b = blockIdx.x / items;
+        const int it = (int)(blockIdx.x - b * items), h0 = it % per_kv * 8 * NT;
+        run_piece<NT>(p, smem, b, it / per_kv, h0, min(8 * NT, p.group - h0), 0, length_of(g, b), nullptr);
+        return;
+    }
+    const int64_t total = units_before(g, g.B, lane) * items;
+    if (total == 0) return;
+    int64_t u = span_of(p, total, blockIdx.x);
+    const int64_t end = span_of(p, total, blockIdx.x + 1);
+    if (u >= end) return;
+    /* the sequence holding unit u: blocks of 32 sequences, then an inclusive scan inside the block */
+    int64_t b = 0, base = 0;
+    for (;; b += 32) {
+        int64_t sum = b + lane < g.B ? units_of(g, b + lane) * items : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += up;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, base + sum > u);
+        if (past) {
+            const int k = __ffs(past) - 1;
+            const int64_t before = __shfl_sync(0xffffffffu, sum, k > 0 ? k - 1 : 0);
+            b += k;
+            base += k > 0 ? before : 0;
+            break;
+        }
+        base += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    Partial<NT>* slots = (Partial<NT>*)p.partials + 2 * (int64_t)blockIdx.x;
+    while (u < end) {
+        const int64_t units = units_of(g, b);
+        if (units > 0) {
+            int64_t rest = u - base;   /* of this sequence's units * items */
+            while (rest < units * items && u < end) {
+                const int it = (int)(rest / units), h0 = it % per_kv * 8 * NT;
+                const int64_t u0 = rest - it * units, n = min(units - u0, end - u), len = length_of(g, b);
+                const bool whole = n == units;
+                run_piece<NT>(p, smem, b, it / per_kv, h0, min(8 * NT, p.group - h0), u0 * kUnit, min((u0 + n) * kUnit, len),
+                              whole ? nullptr : slots + (u0 > 0 ? 0 : 1));
+                u += n;
+                rest += n;
+            }
+            base += units * items;
+        }
+        ++b;
+    }
+}
+
+/* The items the split kernel cut: one CTA a (sequence, query head). The pieces of an item lie in the slots of the CTAs
+ * that own its first to last unit: slot 1 of the first, slot 0 of the others. */
+template <int NT>
+__global__ void __launch_bounds__(128) join_kernel(const Plan p) {
+    __shared__ float om[4][D], ml[4][2];
+    const RidgeFillAttnDecode& g = p.g;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t b = blockIdx.x / g.n_head;
+    const int h = (int)(blockIdx.x - b * g.n_head), in_group = h % p.group;
+    const int items = (int)g.n_head_kv * p.chunks, it = h / p.group * p.chunks + in_group / (8 * NT), row = in_group % (8 * NT);
+    uint16_t* out = g.o + b * g.o_row + (int64_t)h * g.o_head;
+    const int64_t units = units_of(g, b);
+    if (units == 0) {   /* no key: zeros */
+        for (int d = threadIdx.x; d < D / 8; d += 128) *(uint4*)(out + 8 * d) = make_uint4(0u, 0u, 0u, 0u);
+        return;
+    }
+    const int64_t total = units_before(g, g.B, lane) * items;
+    const int64_t start = units_before(g, b, lane) * items + it * units;
+    const int64_t c0 = owner_of(p, total, start), c1 = owner_of(p, total, start + units - 1);
+    if (c0 == c1) return;   /* written by its one CTA */
+    asm volatile("griddepcontrol.wait;" ::: "memory");   /* the split kernel is done and its results are visible */
+    float m = kNone, l = 0.f, acc[8] = {};
+    for (int64_t i = c0 + warp; i <= c1; i += 4) {
+        if (span_of(p, total, i) == span_of(p, total, i + 1)) continue;   /* an empty span left nothing */
+        const Partial<NT>& s = ((const Partial<NT>*)p.partials)[2 * i + (i == c0 ? 1 : 0)];
+        const float sm = s.m[row], up = fmaxf(m, sm);
+        const float f0 = m == kNone ? 0.f : exp2_approx(m - up), f1 = sm == kNone ? 0.f : exp2_approx(sm - up);
+        const float4 x = *(const float4*)&s.o[row][8 * lane], y = *(const float4*)&s.o[row][8 * lane + 4];
+        const float v[8] = { x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w };
+        l = l * f0 + s.l[row] * f1;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = acc[e] * f0 + v[e] * f1;
+        m = up;
+    }
+    if (lane == 0) {
+        ml[warp][0] = m;
+        ml[warp][1] = l;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) om[warp][8 * lane + e] = acc[e];
+    __syncthreads();
+    const float top = fmaxf(fmaxf(ml[0][0], ml[1][0]), fmaxf(ml[2][0], ml[3][0]));
+    const int d = 2 * threadIdx.x;
+    float sum = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float f = ml[i][0] == kNone ? 0.f : exp2_approx(ml[i][0] - top);
+        sum = fmaf(f, ml[i][1], sum);
+        o0 = fmaf(f, om[i][d], o0);
+        o1 = fmaf(f, om[i][d + 1], o1);
+    }
+    const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
+    *(uint32_t*)(out + d) = pack(o0 * inv, o1 * inv);
+}
+
+int sm_count_once() { return rf::sm_count(); }
+
+/* The split of a parsed call: NT (query heads an item / 8), CTAs and scratch bytes (0: one CTA an item). */
+struct Shape {
+    int nt, chunks, ctas;
+    bool split;
+    int64_t bytes;
+};
+Shape shape_of(const RidgeFillAttnDecode& g) {
+    Shape s;
+    const int group = (int)(g.n_head / g.n_head_kv);
+    s.nt = group <= 8 ? 1 : 2;
+    s.chunks = (group + 8 * s.nt - 1) / (8 * s.nt);
+    s.split = g.n_pages * g.page > 2 * kUnit;
+    s.ctas = sm_count_once() * kCtasPerSm;
+    const int64_t one = s.nt == 1 ? (int64_t)sizeof(Partial<1>) : (int64_t)sizeof(Partial<2>);
+    s.bytes = s.split ? 2 * one * s.ctas : 0;
+    return s;
+}
+
+template <int NT>
+int launch(const Plan& p, bool split, cudaStream_t s) {
+    if (cudaFuncSetAttribute(decode_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) {
+        cudaGetLastError();
+        return RAD_E_DEVICE;
+    }
+    const int64_t grid = split ? p.ctas : p.g.B * p.g.n_head_kv * p.chunks;
+    decode_kernel<NT><<<(unsigned)grid, kThreads, kSmem, s>>>(p);
+    if (!split) return rf::launch_status();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.g.B * p.g.n_head));
+    cfg.blockDim = dim3(128);
+    cfg.stream = s;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    const int rc = rf::launch_status();
+    if (rc != RAD_OK) return rc;
+    if (cudaLaunchKernelEx(&cfg, join_kernel<NT>, p) != cudaSuccess) {
+        cudaGetLastError();
+        return RAD_E_DEVICE;
+    }
+    return RAD_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t ridgefill_attn_decode_scratch(const RadArgs* a) {
+    RidgeFillAttnDecode g;
+    return ridgefill_attn_decode_parse(a, &g) == RAD_OK && g.B > 0 ? shape_of(g).bytes : 0;
+}
+
+extern "C" int ridgefill_attn_decode_device(const RadArgs* a, RadStream s) {
+    Plan p;
+    const int rc = ridgefill_attn_decode_parse(a, &p.g);
+    if (rc != RAD_OK) return rc;
+    if (p.g.B == 0) return RAD_OK;
+    if (p.g.B * p.g.n_head > 0x7fffffffLL) return RAD_E_SHAPE;
+    const Shape sh = shape_of(p.g);
+    if (sh.split && (!a->scratch || a->scratch_bytes < sh.bytes || (uintptr_t)a->scratch % 16)) return RAD_E_INVAL;
+    p.group = (int)(p.g.n_head / p.g.n_head_kv);
+    p.chunks = sh.chunks;
+    p.ctas = sh.ctas;
+    p.partials = sh.split ? a->scratch : nullptr;
+    p.scale_log2 = p.g.scale * 1.4426950408889634f;
+    return sh.nt == 1 ? launch<1>(p, sh.split, rf::as_stream(s)) : launch<2>(p, sh.split, rf::as_stream(s));
+}

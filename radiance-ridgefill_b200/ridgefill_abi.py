@@ -141,6 +141,18 @@ def absent() -> RadTensor:
     return RadTensor()
 
 
+class Call:
+    """One row's call with its argument block built once: `call(stream)` is the launch alone. It keeps the descriptors,
+    not the memory they point to."""
+
+    def __init__(self, row: RadKernelInfo, tensors, params, scratch: int | None = None, scratch_bytes: int = 0):
+        self._args, self._keep = Plugin.args(tensors, params, scratch, scratch_bytes)
+        self._launch, self._ref = row.launch, C.byref(self._args)
+
+    def __call__(self, stream: int | None = None) -> int:
+        return self._launch(self._ref, stream)
+
+
 class Plugin:
     """A loaded kernel plugin: its schemas and rows, found by (op, domain) as the engine finds them."""
 
@@ -162,6 +174,12 @@ class Plugin:
         L.rad_kernel_at.argtypes = [C.c_int]
         L.rad_kernel_concurrent.restype = C.c_int
         L.rad_kernel_concurrent.argtypes = [C.c_int]
+        self._serves = hasattr(L, "ridgefill_serve_count")   # the serving rows' own table (include/ridgefill_serve.h)
+        if self._serves:
+            L.ridgefill_serve_schema_at.restype = C.POINTER(RadOpSchema)
+            L.ridgefill_serve_schema_at.argtypes = [C.c_int]
+            L.ridgefill_serve_at.restype = C.POINTER(RadKernelInfo)
+            L.ridgefill_serve_at.argtypes = [C.c_int]
         if L.rad_plugin_abi_version() != RAD_ABI_VERSION:
             raise RuntimeError(f"{path}: ABI {L.rad_plugin_abi_version():#x}, expected {RAD_ABI_VERSION:#x}")
 
@@ -172,8 +190,13 @@ class Plugin:
     def schemas(self) -> list[RadOpSchema]:
         return [self.lib.rad_kernel_schema_at(i).contents for i in range(self.lib.rad_kernel_schema_count())]
 
+    def serve_schemas(self) -> list[RadOpSchema]:
+        """The serving rows' schemas (none in a library without them)."""
+        n = self.lib.ridgefill_serve_schema_count() if self._serves else 0
+        return [self.lib.ridgefill_serve_schema_at(i).contents for i in range(n)]
+
     def schema(self, op: str) -> RadOpSchema | None:
-        for s in self.schemas():
+        for s in self.schemas() + self.serve_schemas():
             if s.op.decode() == op:
                 return s
         return None
@@ -181,8 +204,13 @@ class Plugin:
     def rows(self) -> list[RadKernelInfo]:
         return [self.lib.rad_kernel_at(i).contents for i in range(self.lib.rad_kernel_count())]
 
+    def serve_rows(self) -> list[RadKernelInfo]:
+        """The serving rows: a table of their own beside the plugin's."""
+        n = self.lib.ridgefill_serve_count() if self._serves else 0
+        return [self.lib.ridgefill_serve_at(i).contents for i in range(n)]
+
     def find_row(self, op: str, domain: int) -> RadKernelInfo | None:
-        for r in self.rows():
+        for r in self.rows() + self.serve_rows():
             if r.domain == domain and r.op.decode() == op:
                 return r
         return None
@@ -208,6 +236,10 @@ class Plugin:
         rc = row.launch(C.byref(a), C.c_void_p(stream) if stream else None)
         del keep
         return rc
+
+    def bind(self, row: RadKernelInfo, tensors, params, scratch: int | None = None, scratch_bytes: int = 0) -> Call:
+        """The call of `row` on these operands, for a program that issues it again and again."""
+        return Call(row, tensors, params, scratch, scratch_bytes)
 
     def scratch_bytes(self, row: RadKernelInfo, tensors, params) -> int:
         if not row.scratch:

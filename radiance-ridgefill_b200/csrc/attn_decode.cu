@@ -5,7 +5,7 @@
  * query heads are served from that read. The arithmetic (4 D flops a key and query head) goes through mma.sync, far
  * below its rate. What decides the time is how evenly the bytes spread over the SMs and how many are in flight.
  *
- * Work. A unit is 64 keys of one item (a sequence's kv head and up to 16 of its query heads). The units of all items
+ * Work. A unit is 16 keys of one item (a sequence's kv head and up to 16 of its query heads). The units of all items
  * in order -- sequence, head, position -- are cut into equal spans, one a CTA, whatever the lengths: a long sequence
  * spreads over many CTAs, short ones share one. The lengths are device memory, so every CTA finds its span from
  * kv_lens itself. A span that covers a whole item writes its output; the at most two items a span cuts leave a partial
@@ -34,9 +34,10 @@ namespace {
 constexpr int D = 256;
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kBlock = 16;                          /* keys a warp takes at a time */
-constexpr int kUnit = kWarps * kBlock;              /* keys of a unit */
+constexpr int kRound = kWarps * kBlock;             /* keys the warps of a CTA take together */
 constexpr int kHalfBytes = kBlock * D * 2;          /* a block's keys, or its values */
 constexpr int kRing = 3;                            /* halves of a warp's ring */
+constexpr int kStart = 4;                           /* a piece's fixed cost, in blocks */
 constexpr int kSmem = kWarps * kRing * kHalfBytes;
 constexpr int kCtasPerSm = 2;
 constexpr float kGrow = 8.0f;                       /* a maximum may be exceeded by 2^8 before the sums are rescaled */
@@ -52,24 +53,29 @@ struct Partial {                                    /* one piece's result */
 struct Plan {
     RidgeFillAttnDecode g;
     int group, chunks;      /* query heads a kv head; items a kv head (group / heads of an item, rounded up) */
-    int ctas;               /* CTAs of the split kernel */
+    int ctas, seats;        /* CTAs of the split kernel; how many of them run at a time */
+    bool narrow;            /* its grid has CTAs for narrow spans */
+    int parts;              /* CTAs a query head's join */
     void* partials;         /* [ctas][2] Partial; null: one CTA an item, nothing to join */
     float scale_log2;
 };
 
-__device__ __forceinline__ int64_t length_of(const RidgeFillAttnDecode& g, int64_t b) {
-    const int64_t most = g.n_pages * g.page, n = g.lens[b];
+/* Lengths and units are 32-bit: the host refuses a call whose table could hold more (ridgefill_attn_decode_device). */
+__device__ __forceinline__ int length_of(const RidgeFillAttnDecode& g, int b) {
+    const int most = (int)(g.n_pages * g.page), n = g.lens[b];
     return n < 0 ? 0 : (n > most ? most : n);
 }
-__device__ __forceinline__ int64_t units_of(const RidgeFillAttnDecode& g, int64_t b) { return (length_of(g, b) + kUnit - 1) / kUnit; }
+/* The units of an item of sequence b: kStart for its beginning (what a piece costs beside its keys: its first copies'
+ * latency, the warps' meeting at its end), then one a block; none without keys. */
+__device__ __forceinline__ int units_of(const RidgeFillAttnDecode& g, int b) {
+    const int len = length_of(g, b);
+    return len ? kStart + (len + kBlock - 1) / kBlock : 0;
+}
 
-/* Units of sequences [0, n) of one kv head and chunk; the whole warp. */
-__device__ __forceinline__ int64_t units_before(const RidgeFillAttnDecode& g, int64_t n, int lane) {
-    int64_t sum = 0;
-    for (int64_t b = lane; b < n; b += 32) sum += units_of(g, b);
+__device__ __forceinline__ int warp_sum(int x) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sum;
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -92,15 +98,15 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 /* One warp's walk over the 16-key blocks of a piece. */
 struct Blocks {
     const uint16_t* keys;      /* cache plane 0 at the item's kv head */
-    int64_t len;               /* the sequence's keys */
+    int len;                   /* the sequence's keys */
     const int32_t* table;      /* its pages */
 };
 
 /* The slot of key `j` (-1: past the sequence, or outside the pool), by the lane that owns it. */
-__device__ __forceinline__ int slot_of(const RidgeFillAttnDecode& g, const Blocks& w, int64_t j) {
+__device__ __forceinline__ int slot_of(const RidgeFillAttnDecode& g, const Blocks& w, int j) {
     if (j >= w.len) return -1;
-    const int page = (int)g.page, n = (int)j / page;
-    const int64_t slot = (int64_t)w.table[n] * page + ((int)j - n * page);
+    const int page = (int)g.page, n = j / page;
+    const int64_t slot = (int64_t)w.table[n] * page + (j - n * page);
     return slot >= 0 && slot < g.n_slots ? (int)slot : -1;
 }
 
@@ -113,8 +119,8 @@ __device__ __forceinline__ void fetch(const RidgeFillAttnDecode& g, const Blocks
         const uint16_t* p1 = w.keys + (int64_t)max(s1, 0) * g.c_slot + 8 * c;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
-            rf::cp_async16(half + (2 * j) * 512 + lane * 16, p0 + 32 * j, s0 >= 0 ? 16 : 0);
-            rf::cp_async16(half + (2 * j + 1) * 512 + lane * 16, p1 + 32 * j, s1 >= 0 ? 16 : 0);
+            rf::cp_async16_l2(half + (2 * j) * 512 + lane * 16, p0 + 32 * j, s0 >= 0 ? 16 : 0);
+            rf::cp_async16_l2(half + (2 * j + 1) * 512 + lane * 16, p1 + 32 * j, s1 >= 0 ? 16 : 0);
         }
     } else {
 #pragma unroll
@@ -122,7 +128,7 @@ __device__ __forceinline__ void fetch(const RidgeFillAttnDecode& g, const Blocks
             const int s = __shfl_sync(0xffffffffu, slots, 2 * c + (i & 1) + (i >> 1) * 8);
             const uint16_t* p = w.keys + g.c_kv + (int64_t)max(s, 0) * g.c_slot + 8 * r;
 #pragma unroll
-            for (int j = 0; j < D / 64; ++j) rf::cp_async16(half + (4 * j + i) * 512 + lane * 16, p + 64 * j, s >= 0 ? 16 : 0);
+            for (int j = 0; j < D / 64; ++j) rf::cp_async16_l2(half + (4 * j + i) * 512 + lane * 16, p + 64 * j, s >= 0 ? 16 : 0);
         }
     }
     rf::cp_async_commit();
@@ -131,14 +137,14 @@ __device__ __forceinline__ void fetch(const RidgeFillAttnDecode& g, const Blocks
 /* A piece's keys [from, to) of item (b, kv head, first query head h0, heads), by the whole CTA; its result to the
  * output (`out`) or to `part`. */
 template <int NT>
-__device__ __forceinline__ void run_piece(const Plan& p, uint8_t* smem, int64_t b, int64_t hkv, int h0, int heads, int64_t from,
-                                          int64_t to, Partial<NT>* part) {
+__device__ __forceinline__ void run_piece(const Plan& p, uint8_t* smem, int b, int hkv, int h0, int heads, int from, int to,
+                                          Partial<NT>* part) {
     const RidgeFillAttnDecode& g = p.g;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
     uint8_t* ring = smem + warp * kRing * kHalfBytes;
     const Blocks w = { g.cache + hkv * g.c_head, length_of(g, b), g.table + b * g.t_row };
-    const int64_t first = from + warp * kBlock;
-    const int n = first < to ? (int)((to - first + kUnit - 1) / kUnit) : 0;   /* this warp's blocks */
+    const int first = from + warp * kBlock;
+    const int n = first < to ? (to - first + kRound - 1) / kRound : 0;   /* this warp's blocks */
 
     float o[NT][D / 16][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -153,7 +159,7 @@ __device__ __forceinline__ void run_piece(const Plan& p, uint8_t* smem, int64_t 
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int h = 8 * t + r;
-        const uint16_t* src = g.q + b * g.q_row + (hkv * p.group + h0 + h) * g.q_head + 8 * c;
+        const uint16_t* src = g.q + b * g.q_row + (int64_t)(hkv * p.group + h0 + h) * g.q_head + 8 * c;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) q[t][j] = h < heads ? *(const uint4*)(src + 32 * j) : make_uint4(0u, 0u, 0u, 0u);
     }
@@ -161,13 +167,13 @@ __device__ __forceinline__ void run_piece(const Plan& p, uint8_t* smem, int64_t 
     int cur = -1, next = -1;   /* lanes 0..15: the slots of blocks i and i + 1 */
     if (n > 0) {
         cur = slot_of(g, w, first + (lane & 15));
-        next = n > 1 ? slot_of(g, w, first + kUnit + (lane & 15)) : -1;
+        next = n > 1 ? slot_of(g, w, first + kRound + (lane & 15)) : -1;
         fetch(g, w, cur, false, ring, lane);
         fetch(g, w, cur, true, ring + kHalfBytes, lane);
     }
     int at = 0;   /* ring slot of the current half */
     for (int i = 0; i < n; ++i) {
-        const int after = i + 2 < n ? slot_of(g, w, first + (int64_t)(i + 2) * kUnit + (lane & 15)) : -1;
+        const int after = i + 2 < n ? slot_of(g, w, first + (i + 2) * kRound + (lane & 15)) : -1;
         /* scores of the block's 16 keys */
         int free_slot = at + 2 >= kRing ? at + 2 - kRing : at + 2;
         if (i + 1 < n) fetch(g, w, next, false, ring + free_slot * kHalfBytes, lane);
@@ -316,16 +322,46 @@ __device__ __forceinline__ void run_piece(const Plan& p, uint8_t* smem, int64_t 
             }
         } else {
             const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);   /* no key: zeros; a NaN stays one */
-            *(uint2*)(g.o + b * g.o_row + (hkv * p.group + h0 + h) * g.o_head + d) =
+            *(uint2*)(g.o + b * g.o_row + (int64_t)(hkv * p.group + h0 + h) * g.o_head + d) =
                 make_uint2(pack(acc.x * inv, acc.y * inv), pack(acc.z * inv, acc.w * inv));
         }
     }
     __syncthreads();   /* the results are read before the next piece's copies land */
 }
 
-/* CTA i's first unit of `total`; the CTA whose span holds unit u. */
-__device__ __forceinline__ int64_t span_of(const Plan& p, int64_t total, int64_t i) { return i * total / p.ctas; }
-__device__ __forceinline__ int64_t owner_of(const Plan& p, int64_t total, int64_t u) { return ((u + 1) * p.ctas - 1) / total; }
+/* The units cut into spans, CTA i taking span i. `seats` CTAs run at a time.
+ * With few units: as many CTAs as have one for each of their warps, at most one a seat, equal spans.
+ * From kLong units a seat on: SMs do not get equal shares of the memory's rate, so equal spans leave some idle at the
+ * end (13 % of the SMs' time at 64 sequences of up to 32,768). One wide span a seat takes 4/5 of the units, and four
+ * times as many narrow ones follow, which the hardware gives to whichever seat comes free. */
+constexpr int kLong = 128, kNarrowPerSeat = 4;
+struct Spans {
+    int n_wide = 0, wide = 0, n = 0, each = 0, extra = 0;   /* n equal spans after the wide ones, the first `extra` one longer */
+    __device__ __forceinline__ Spans(int total, int seats, bool narrow) {
+        if (narrow && total / kLong >= seats) {
+            n_wide = seats;
+            wide = total / seats * 4 / 5;
+            n = kNarrowPerSeat * seats;
+        } else {
+            n = min((total + kWarps - 1) / kWarps, seats);
+        }
+        const int rest = total - n_wide * wide;
+        each = rest / n;
+        extra = rest - each * n;
+    }
+    __device__ __forceinline__ int ctas() const { return n_wide + n; }
+    __device__ __forceinline__ int first(int i) const {
+        if (i <= n_wide) return i * wide;
+        i -= n_wide;
+        return n_wide * wide + i * each + min(i, extra);
+    }
+    __device__ __forceinline__ int owner(int u) const {
+        if (u < n_wide * wide) return u / wide;
+        u -= n_wide * wide;
+        const int longer = extra * (each + 1);
+        return n_wide + (u < longer ? u / (each + 1) : extra + (u - longer) / each);
+    }
+};
 
 template <int NT>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Plan p) {
@@ -335,29 +371,32 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Plan
     const int per_kv = p.chunks, items = (int)g.n_head_kv * per_kv;   /* items of a sequence */
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   /* the join may take its place on the SMs */
     if (!p.partials) {   /* one CTA an item */
-        const int64_t b = blockIdx.x / items;
-        const int it = (int)(blockIdx.x - b * items), h0 = it % per_kv * 8 * NT;
+        const int b = blockIdx.x / items, it = blockIdx.x - b * items, h0 = it % per_kv * 8 * NT;
         run_piece<NT>(p, smem, b, it / per_kv, h0, min(8 * NT, p.group - h0), 0, length_of(g, b), nullptr);
         return;
     }
-    const int64_t total = units_before(g, g.B, lane) * items;
+    const int B = (int)g.B;
+    int total = 0;
+    for (int i = lane; i < B; i += 32) total += units_of(g, i);
+    total = warp_sum(total) * items;
     if (total == 0) return;
-    int64_t u = span_of(p, total, blockIdx.x);
-    const int64_t end = span_of(p, total, blockIdx.x + 1);
-    if (u >= end) return;
+    const Spans spans(total, p.seats, p.narrow);
+    if ((int)blockIdx.x >= spans.ctas()) return;
+    int u = spans.first(blockIdx.x);
+    const int end = spans.first(blockIdx.x + 1);
     /* the sequence holding unit u: blocks of 32 sequences, then an inclusive scan inside the block */
-    int64_t b = 0, base = 0;
+    int b = 0, base = 0;
     for (;; b += 32) {
-        int64_t sum = b + lane < g.B ? units_of(g, b + lane) * items : 0;
+        int sum = b + lane < B ? units_of(g, b + lane) * items : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+            const int up = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += up;
         }
         const unsigned past = __ballot_sync(0xffffffffu, base + sum > u);
         if (past) {
             const int k = __ffs(past) - 1;
-            const int64_t before = __shfl_sync(0xffffffffu, sum, k > 0 ? k - 1 : 0);
+            const int before = __shfl_sync(0xffffffffu, sum, k > 0 ? k - 1 : 0);
             b += k;
             base += k > 0 ? before : 0;
             break;
@@ -366,15 +405,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Plan
     }
     Partial<NT>* slots = (Partial<NT>*)p.partials + 2 * (int64_t)blockIdx.x;
     while (u < end) {
-        const int64_t units = units_of(g, b);
+        const int units = units_of(g, b);
         if (units > 0) {
-            int64_t rest = u - base;   /* of this sequence's units * items */
+            int rest = u - base;   /* of this sequence's units * items */
             while (rest < units * items && u < end) {
-                const int it = (int)(rest / units), h0 = it % per_kv * 8 * NT;
-                const int64_t u0 = rest - it * units, n = min(units - u0, end - u), len = length_of(g, b);
-                const bool whole = n == units;
-                run_piece<NT>(p, smem, b, it / per_kv, h0, min(8 * NT, p.group - h0), u0 * kUnit, min((u0 + n) * kUnit, len),
-                              whole ? nullptr : slots + (u0 > 0 ? 0 : 1));
+                const int it = rest / units, h0 = it % per_kv * 8 * NT;
+                const int u0 = rest - it * units, n = min(units - u0, end - u), len = length_of(g, b);
+                const int first = max(u0 - kStart, 0), last = u0 + n - kStart;   /* blocks; none: the item begins in the next span */
+                if (last > 0)
+                    run_piece<NT>(p, smem, b, it / per_kv, h0, min(8 * NT, p.group - h0), first * kBlock, min(last * kBlock, len),
+                                  first == 0 && u0 + n == units ? nullptr : slots + (first > 0 ? 0 : 1));
                 u += n;
                 rest += n;
             }
@@ -384,67 +424,90 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Plan
     }
 }
 
-/* The items the split kernel cut: one CTA a (sequence, query head). The pieces of an item lie in the slots of the CTAs
- * that own its first to last unit: slot 1 of the first, slot 0 of the others. */
+constexpr int kJoinThreads = 256, kJoinFlight = 8;
+
+/* The items the split kernel cut. The pieces of an item lie in the slots of the CTAs that own its first to last block:
+ * slot 1 of the first, slot 0 of the others. A CTA joins D / p.parts elements of one query head of a sequence: groups of
+ * threads, four elements a thread, take every so-many-th piece, kJoinFlight pieces' loads in flight, with a running
+ * maximum of their own, and meet at the end. */
 template <int NT>
-__global__ void __launch_bounds__(128) join_kernel(const Plan p) {
-    __shared__ float om[4][D], ml[4][2];
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Plan p) {
+    __shared__ float4 sums[kJoinThreads];
+    __shared__ float2 stats[kJoinThreads];
     const RidgeFillAttnDecode& g = p.g;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t b = blockIdx.x / g.n_head;
-    const int h = (int)(blockIdx.x - b * g.n_head), in_group = h % p.group;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int n_head = (int)g.n_head, B = (int)g.B;
+    const int part = blockIdx.x % p.parts, bh = blockIdx.x / p.parts;
+    const int b = bh / n_head, h = bh - b * n_head, in_group = h % p.group;
     const int items = (int)g.n_head_kv * p.chunks, it = h / p.group * p.chunks + in_group / (8 * NT), row = in_group % (8 * NT);
-    uint16_t* out = g.o + b * g.o_row + (int64_t)h * g.o_head;
-    const int64_t units = units_of(g, b);
+    const int lanes = D / 4 / p.parts, groups = kJoinThreads / lanes, group = tid / lanes, d = (part * lanes + tid % lanes) * 4;
+    uint16_t* out = g.o + b * g.o_row + (int64_t)h * g.o_head + d;
+    const int units = units_of(g, b);
     if (units == 0) {   /* no key: zeros */
-        for (int d = threadIdx.x; d < D / 8; d += 128) *(uint4*)(out + 8 * d) = make_uint4(0u, 0u, 0u, 0u);
+        if (group == 0) *(uint2*)out = make_uint2(0u, 0u);
         return;
     }
-    const int64_t total = units_before(g, g.B, lane) * items;
-    const int64_t start = units_before(g, b, lane) * items + it * units;
-    const int64_t c0 = owner_of(p, total, start), c1 = owner_of(p, total, start + units - 1);
-    if (c0 == c1) return;   /* written by its one CTA */
+    int total = 0, before = 0;
+    for (int i = lane; i < B; i += 32) {
+        const int n = units_of(g, i);
+        total += n;
+        before += i < b ? n : 0;
+    }
+    const Spans spans(warp_sum(total) * items, p.seats, p.narrow);
+    const int start = warp_sum(before) * items + it * units;
+    const int c0 = spans.owner(start + kStart), n = spans.owner(start + units - 1) - c0 + 1;
+    if (n == 1) return;   /* written by its one CTA */
     asm volatile("griddepcontrol.wait;" ::: "memory");   /* the split kernel is done and its results are visible */
-    float m = kNone, l = 0.f, acc[8] = {};
-    for (int64_t i = c0 + warp; i <= c1; i += 4) {
-        if (span_of(p, total, i) == span_of(p, total, i + 1)) continue;   /* an empty span left nothing */
-        const Partial<NT>& s = ((const Partial<NT>*)p.partials)[2 * i + (i == c0 ? 1 : 0)];
-        const float sm = s.m[row], up = fmaxf(m, sm);
-        const float f0 = m == kNone ? 0.f : exp2_approx(m - up), f1 = sm == kNone ? 0.f : exp2_approx(sm - up);
-        const float4 x = *(const float4*)&s.o[row][8 * lane], y = *(const float4*)&s.o[row][8 * lane + 4];
-        const float v[8] = { x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w };
-        l = l * f0 + s.l[row] * f1;
+    const Partial<NT>* pieces = (const Partial<NT>*)p.partials + 2 * (int64_t)c0;
+    float m = kNone, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = group; i0 < n; i0 += kJoinFlight * groups) {
+        float pm[kJoinFlight], pl[kJoinFlight];
+        float4 po[kJoinFlight];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = acc[e] * f0 + v[e] * f1;
+        for (int k = 0; k < kJoinFlight; ++k) {
+            const int i = i0 + k * groups;
+            const Partial<NT>& s = pieces[2 * min(i, n - 1) + (i == 0 ? 1 : 0)];
+            pm[k] = i < n ? s.m[row] : kNone;
+            pl[k] = i < n ? s.l[row] : 0.f;
+            po[k] = i < n ? *(const float4*)&s.o[row][d] : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float up = m;
+#pragma unroll
+        for (int k = 0; k < kJoinFlight; ++k) up = fmaxf(up, pm[k]);
+        const float f = m == kNone ? 0.f : exp2_approx(m - up);
+        l *= f;
+        acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+#pragma unroll
+        for (int k = 0; k < kJoinFlight; ++k) {
+            const float w = pm[k] == kNone ? 0.f : exp2_approx(pm[k] - up);
+            l = fmaf(w, pl[k], l);
+            acc = make_float4(fmaf(w, po[k].x, acc.x), fmaf(w, po[k].y, acc.y), fmaf(w, po[k].z, acc.z), fmaf(w, po[k].w, acc.w));
+        }
         m = up;
     }
-    if (lane == 0) {
-        ml[warp][0] = m;
-        ml[warp][1] = l;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) om[warp][8 * lane + e] = acc[e];
+    sums[tid] = acc;
+    stats[tid] = make_float2(m, l);
     __syncthreads();
-    const float top = fmaxf(fmaxf(ml[0][0], ml[1][0]), fmaxf(ml[2][0], ml[3][0]));
-    const int d = 2 * threadIdx.x;
-    float sum = 0.f, o0 = 0.f, o1 = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float f = ml[i][0] == kNone ? 0.f : exp2_approx(ml[i][0] - top);
-        sum = fmaf(f, ml[i][1], sum);
-        o0 = fmaf(f, om[i][d], o0);
-        o1 = fmaf(f, om[i][d + 1], o1);
+    if (group > 0) return;
+    float top = kNone, sum = 0.f;
+    for (int k = 0; k < groups; ++k) top = fmaxf(top, stats[tid + k * lanes].x);
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < groups; ++k) {
+        const float2 s = stats[tid + k * lanes];
+        const float4 v = sums[tid + k * lanes];
+        const float w = s.x == kNone ? 0.f : exp2_approx(s.x - top);
+        sum = fmaf(w, s.y, sum);
+        acc = make_float4(fmaf(w, v.x, acc.x), fmaf(w, v.y, acc.y), fmaf(w, v.z, acc.z), fmaf(w, v.w, acc.w));
     }
     const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
-    *(uint32_t*)(out + d) = pack(o0 * inv, o1 * inv);
+    *(uint2*)out = make_uint2(pack(acc.x * inv, acc.y * inv), pack(acc.z * inv, acc.w * inv));
 }
-
-int sm_count_once() { return rf::sm_count(); }
 
 /* The split of a parsed call: NT (query heads an item / 8), CTAs and scratch bytes (0: one CTA an item). */
 struct Shape {
-    int nt, chunks, ctas;
-    bool split;
+    int nt, chunks, ctas, seats;
+    bool split, narrow;
     int64_t bytes;
 };
 Shape shape_of(const RidgeFillAttnDecode& g) {
@@ -452,8 +515,11 @@ Shape shape_of(const RidgeFillAttnDecode& g) {
     const int group = (int)(g.n_head / g.n_head_kv);
     s.nt = group <= 8 ? 1 : 2;
     s.chunks = (group + 8 * s.nt - 1) / (8 * s.nt);
-    s.split = g.n_pages * g.page > 2 * kUnit;
-    s.ctas = sm_count_once() * kCtasPerSm;
+    s.split = g.n_pages * g.page > 2 * kRound;
+    s.seats = rf::sm_count() * kCtasPerSm;
+    /* whether the tables could hold enough for narrow spans; whether the lengths do is the kernels' to see */
+    s.narrow = g.B * g.n_head_kv * s.chunks * (g.n_pages * g.page / kBlock + 1 + kStart) / kLong >= s.seats;
+    s.ctas = s.narrow ? (1 + kNarrowPerSeat) * s.seats : s.seats;
     const int64_t one = s.nt == 1 ? (int64_t)sizeof(Partial<1>) : (int64_t)sizeof(Partial<2>);
     s.bytes = s.split ? 2 * one * s.ctas : 0;
     return s;
@@ -469,8 +535,8 @@ int launch(const Plan& p, bool split, cudaStream_t s) {
     decode_kernel<NT><<<(unsigned)grid, kThreads, kSmem, s>>>(p);
     if (!split) return rf::launch_status();
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(p.g.B * p.g.n_head));
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3((unsigned)(p.g.B * p.g.n_head * p.parts));
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = s;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -498,12 +564,17 @@ extern "C" int ridgefill_attn_decode_device(const RadArgs* a, RadStream s) {
     const int rc = ridgefill_attn_decode_parse(a, &p.g);
     if (rc != RAD_OK) return rc;
     if (p.g.B == 0) return RAD_OK;
-    if (p.g.B * p.g.n_head > 0x7fffffffLL) return RAD_E_SHAPE;
+    /* grids, and the units of all items, in 32 bits */
+    if (p.g.B > 0x7fffffffLL / p.g.n_head || p.g.B * p.g.n_head * (p.g.n_pages * p.g.page / kBlock + 1 + kStart) > 0x7fffffffLL) return RAD_E_SHAPE;
     const Shape sh = shape_of(p.g);
     if (sh.split && (!a->scratch || a->scratch_bytes < sh.bytes || (uintptr_t)a->scratch % 16)) return RAD_E_INVAL;
     p.group = (int)(p.g.n_head / p.g.n_head_kv);
     p.chunks = sh.chunks;
     p.ctas = sh.ctas;
+    p.seats = sh.seats;
+    p.narrow = sh.narrow;
+    /* few heads have many pieces each: four CTAs a head share them (29 -> 26 us for one sequence of 32,768) */
+    p.parts = p.g.B * p.g.n_head <= sh.seats ? 4 : 1;
     p.partials = sh.split ? a->scratch : nullptr;
     p.scale_log2 = p.g.scale * 1.4426950408889634f;
     return sh.nt == 1 ? launch<1>(p, sh.split, rf::as_stream(s)) : launch<2>(p, sh.split, rf::as_stream(s));

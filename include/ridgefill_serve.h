@@ -18,10 +18,31 @@
 
 #include "ridgefill.h"
 
-/* ridgefill_attn_decode: operand positions. */
+/* Operand positions. ridgefill_attn_prefill: */
+enum { AP_Q = 0, AP_K, AP_V, AP_CU_Q, AP_CU_K, AP_O };
+/* ridgefill_attn_decode */
 enum { AD_Q = 0, AD_CACHE, AD_TABLE, AD_LENS, AD_O };
 /* ridgefill_gdn_step */
 enum { GS_Q = 0, GS_K, GS_V, GS_G, GS_BETA, GS_STATE, GS_STATE_IDX, GS_OUT_IDX, GS_O };
+
+/* ridgefill_attn_prefill: causal attention over packed prompts. Sequence i holds the rows [cu_q[i], cu_q[i+1]) of q and
+ * the rows [cu_k[i], cu_k[i+1]) of k and v (cu_q's without cu_k); with nq and nk of them, row r (0 <= r < nq) sees the
+ * keys 0 .. nk - nq + r: the queries are the sequence's last rows, all of a prompt or its tail. Query head h reads kv
+ * head h / (Hq / Hkv):
+ *     o[r, h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q[r, h] . k_j)
+ * zeros for a row that sees no key; rows outside every sequence are not written. The products q . k are exact bf16
+ * products summed in f32; p is rounded to bf16 for the product with v and summed in f32; o is rounded once. A value of v
+ * that is not finite reaches the rows that see it and may reach earlier rows of its own sequence, up to 127 keys before
+ * it (they share its key tile, where its weight for them is zero); no row of another sequence. */
+typedef struct RidgeFillAttnPrefill {
+    const uint16_t* q;       int64_t q_row, q_head;              /* [T, Hq, D] */
+    const uint16_t* k;       int64_t k_row, k_head;              /* [Tk, Hkv, D] */
+    const uint16_t* v;       int64_t v_row, v_head;              /* [Tk, Hkv, D] */
+    const int32_t*  cu_q;    const int32_t* cu_k;                /* [n_seq + 1] */
+    uint16_t*       o;       int64_t o_row, o_head;              /* [T, Hq, D] */
+    int64_t         T, Tk, n_seq, n_head, n_head_kv, head_dim;
+    float           scale;
+} RidgeFillAttnPrefill;
 
 /* ridgefill_attn_decode: one new token a sequence over the paged cache. Sequence i's key j (0 <= j < lens[i]) lies in
  * slot table[i, j / page] * page + j % page of cache [2, slots, Hkv, D]; query head h reads kv head h / (Hq / Hkv):
@@ -70,10 +91,12 @@ const RadKernelInfo* ridgefill_serve_at(int i);
 
 /* Parses: RAD_OK or a named refusal (null operands and missing parameters RAD_E_INVAL, types RAD_E_DTYPE, ranks and
  * extents RAD_E_SHAPE, strides and alignment RAD_E_STRIDE, geometry no kernel serves RAD_E_UNSUPPORTED). */
+int ridgefill_attn_prefill_parse(const RadArgs* a, RidgeFillAttnPrefill* out);
 int ridgefill_attn_decode_parse(const RadArgs* a, RidgeFillAttnDecode* out);
 int ridgefill_gdn_step_parse(const RadArgs* a, RidgeFillGdnStep* out);
 
 /* The device rows: async launches on `s` (a cudaStream_t); no allocation, no synchronisation. */
+int ridgefill_attn_prefill_device(const RadArgs* a, RadStream s);
 int ridgefill_attn_decode_device(const RadArgs* a, RadStream s);
 int ridgefill_gdn_step_device(const RadArgs* a, RadStream s);
 

@@ -23,7 +23,7 @@ OUT = HERE / "ridgefill.so"
 BUILD = HERE / "_build"
 
 CUDA_SOURCES = ["small_ops.cu", "mask.cu", "gemm_q.cu", "gdn.cu", "conv_prep.cu", "attn_kv.cu", "peer.cu", "gdn_step.cu",
-                "attn_decode.cu"]
+                "attn_decode.cu", "attn_prefill.cu"]
 HOST_SOURCES = ["parse.cpp", "rows.cpp", "folder.cpp", "serve_rows.cpp"]
 HEADERS = ["common.cuh", "sm100.cuh", "mma.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

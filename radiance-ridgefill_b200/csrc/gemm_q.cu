@@ -1205,7 +1205,8 @@ extern "C" int ridgefill_quant_act_device(const RadArgs* a, RadStream s) {
 /* The first device-side wait error any kernel of this library recorded (0: none), optionally
  * clearing it. Synchronises the current device: a diagnostic, never called on the launch path. */
 extern "C" int ridgefill_device_error(int reset) {
-    const int gemm = rf::read_device_error(reset), fill = rf::gdn_device_error(reset), team = rf::peer_device_error(reset);
-    if (gemm < 0 || fill < 0 || team < 0) return -1;
-    return gemm ? gemm : fill ? fill : team;
+    const int gemm = rf::read_device_error(reset), fill = rf::gdn_device_error(reset), team = rf::peer_device_error(reset),
+              attn = rf::attn_device_error(reset);
+    if (gemm < 0 || fill < 0 || team < 0 || attn < 0) return -1;
+    return gemm ? gemm : fill ? fill : team ? team : attn;
 }

@@ -41,15 +41,18 @@ int slot_rows(const RadTensor* t, int64_t n, int64_t* pitch) {
     return RAD_OK;
 }
 
-/* The optional `scale` parameter: 1 / sqrt(d) unless given; false when it is not a finite number. */
-bool scale_of(const RadArgs* a, int64_t d, float* out) {
+/* The optional `scale` parameter: 1 / sqrt(d) unless given; false when it is not a finite number (`positive`: above 0). */
+bool scale_of(const RadArgs* a, int64_t d, bool positive, float* out) {
     const double s = rad_args_getf_or(a, "scale", 1.0 / std::sqrt((double)d));
     *out = (float)s;
-    return std::isfinite(*out);
+    return std::isfinite(*out) && (*out > 0.0f || !positive);
 }
 
 /* ------------------------------------------------------------------ schemas */
 
+const RadParamSpec pPrefill[] = { RF_P_INT("M"), RF_P_INT("n_head"), RF_P_INT("n_head_kv"), RF_P_INT("head_dim"),
+                                  RF_P_OPT("scale", RAD_P_F64) };
+const RadOperandSpec oPrefill[] = { RF_IN("q"), RF_IN("k"), RF_IN("v"), RF_IN("cu_seqlens"), RF_IN_OPT("cu_keys"), RF_OUT("o") };
 const RadParamSpec pDecode[] = { RF_P_INT("M"), RF_P_INT("n_head"), RF_P_INT("n_head_kv"), RF_P_INT("head_dim"),
                                  RF_P_INT("page"), RF_P_OPT("scale", RAD_P_F64) };
 const RadOperandSpec oDecode[] = { RF_IN("q"), RF_IN("kv_cache"), RF_IN("block_table"), RF_IN("kv_lens"), RF_OUT("o") };
@@ -59,12 +62,19 @@ const RadOperandSpec oStep[] = { RF_IN("q"), RF_IN("k"), RF_IN("v"), RF_IN("g"),
                                  RF_IN("state_idx"), RF_IN_OPT("out_idx"), RF_OUT("o") };
 
 const RadOpSchema kServeSchemas[] = {
+{ "ridgefill_attn_prefill", RF_ARR(pPrefill), RF_ARR(oPrefill),
+  "Causal attention over packed prompts: sequence i holds rows [cu_seqlens[i], cu_seqlens[i + 1]) of q and rows "
+  "[cu_keys[i], cu_keys[i + 1]) of k and v (cu_seqlens' without cu_keys); with nq and nk of them, row r and query head h "
+  "(kv head h / (n_head / n_head_kv)) give o = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q . k_j), over the keys j <= "
+  "nk - nq + r (the queries are the sequence's last rows); zeros for a row that sees no key, rows outside every sequence "
+  "are not written. scale 1 / sqrt(head_dim) unless given, above 0. q and o bf16 [M, n_head, head_dim], k and v bf16 "
+  "[keys, n_head_kv, head_dim]. head_dim 256." },
 { "ridgefill_attn_decode", RF_ARR(pDecode), RF_ARR(oDecode),
   "Attention of one new token a sequence over the paged cache ridgefill_attn_kv_fill writes: for sequence i (M of them) "
   "and query head h (kv head h / (n_head / n_head_kv)), o[i, h] = sum_j p_j v_j / sum_j p_j with p_j = exp(scale "
   "q[i, h] . k_j) over j < kv_lens[i] (clamped into [0, n_pages * page]), key j in slot block_table[i, j / page] * page "
   "+ j % page of kv_cache bf16 [2, slots, n_head_kv, head_dim]; keys whose slot lies outside the pool are left out, and "
-  "a row without any key is zero. scale 1 / sqrt(head_dim) unless given. q and o bf16 [M, n_head, head_dim], block_table "
+  "a row without any key is zero. scale 1 / sqrt(head_dim) unless given, above 0. q and o bf16 [M, n_head, head_dim], block_table "
   "i32 [M, n_pages], kv_lens i32 [M]. head_dim 256." },
 { "ridgefill_gdn_step", RF_ARR(pStep), RF_ARR(oStep),
   "The gated delta rule for one new token a row (ridgefill_gdn_fill's rule on one-row sequences): per row i of M and "
@@ -76,6 +86,12 @@ const RadOpSchema kServeSchemas[] = {
 };
 
 /* ------------------------------------------------------------------ cold-call descriptions */
+
+int shape_prefill(const RadParam* p, int n_p, int operand, RadOpdDesc* out) {
+    const int64_t T = dim(p, n_p, "M"), h = dim(p, n_p, "n_head"), hkv = dim(p, n_p, "n_head_kv"), D = dim(p, n_p, "head_dim");
+    return pick(out, operand, { opd(RAD_BF16, { T, h, D }), opd(RAD_BF16, { T, hkv, D }), opd(RAD_BF16, { T, hkv, D }),
+                                opd_idx({ 2 }, T, RAD_OPD_F_IDX_CU), opd_absent(), opd(RAD_BF16, { T, h, D }) });
+}
 
 int shape_decode(const RadParam* p, int n_p, int operand, RadOpdDesc* out) {
     const int64_t B = dim(p, n_p, "M"), h = dim(p, n_p, "n_head"), hkv = dim(p, n_p, "n_head_kv");
@@ -100,6 +116,11 @@ int shape_step(const RadParam* p, int n_p, int operand, RadOpdDesc* out) {
       nullptr, scratchfn, nullptr, shapefn, nullptr, nullptr, nullptr, nullptr }
 
 const RadKernelInfo kServeRows[] = {
+    SERVE_ROW("ridgefill_attn_prefill_sm100", "ridgefill_attn_prefill",
+              "tcgen05 kind::f16 into tensor memory, TMA-fed: 128 rows (all query heads of a kv head side by side) x 128 keys a "
+              "tile, the weights back into tensor memory as the second product's operand, persistent CTAs, longest tiles first",
+              "head_dim 256, up to 128 query heads a kv head", "bf16 q / k / v / o, i32 cu_seqlens / cu_keys",
+              ridgefill_attn_prefill_device, nullptr, shape_prefill),
     SERVE_ROW("ridgefill_attn_decode_sm100", "ridgefill_attn_decode",
               "the keys of all sequences split evenly over the SMs, each warp streaming its 16-key blocks through its own "
               "shared-memory ring into mma.sync; the pieces of a sequence joined by a second kernel",
@@ -124,6 +145,60 @@ extern "C" const RadKernelInfo* ridgefill_serve_at(int i) {
 
 /* ------------------------------------------------------------------ parses */
 
+/* ridgefill_attn_prefill: q and o bf16 [T, Hq, 256], k and v bf16 [Tk, Hkv, 256] (dense head rows, bases and other strides
+ * multiples of 16 bytes; q, k and v are read through tensor maps: strides positive and below 2^40 bytes), cu_seqlens and
+ * cu_keys i32 [n_seq + 1] dense. Hq a multiple of Hkv, at most 128 query heads a kv head. */
+extern "C" int ridgefill_attn_prefill_parse(const RadArgs* a, RidgeFillAttnPrefill* g) {
+    *g = RidgeFillAttnPrefill{};
+    const RadTensor* Q = rad_arg_in(a, AP_Q);
+    const RadTensor* K = rad_arg_in(a, AP_K);
+    const RadTensor* V = rad_arg_in(a, AP_V);
+    const RadTensor* CQ = rad_arg_in(a, AP_CU_Q);
+    const RadTensor* CK = rad_arg_in(a, AP_CU_K);
+    const RadTensor* O = rad_arg_in(a, AP_O);
+    long long T = 0, h = 0, hkv = 0, D = 0;
+    if (!Q || !K || !V || !CQ || !O || !rad_args_geti(a, "M", &T) || !rad_args_geti(a, "n_head", &h) ||
+        !rad_args_geti(a, "n_head_kv", &hkv) || !rad_args_geti(a, "head_dim", &D))
+        return RAD_E_INVAL;
+    if (D != 256) return RAD_E_UNSUPPORTED;
+    if (!scale_of(a, D, true, &g->scale)) return RAD_E_INVAL;
+    if (Q->dtype != RAD_BF16 || K->dtype != RAD_BF16 || V->dtype != RAD_BF16 || O->dtype != RAD_BF16 || CQ->dtype != RAD_I32 ||
+        (CK && CK->dtype != RAD_I32))
+        return RAD_E_DTYPE;
+    if (T < 0 || h <= 0 || hkv <= 0) return RAD_E_SHAPE;
+    if (h % hkv != 0 || h / hkv > 128) return RAD_E_UNSUPPORTED;
+    const int64_t most = 0x7ffffe00LL;   /* rows, with a tile's to spare, in 32 bits */
+    if (!is(Q, { T, h, D }) || !is(O, { T, h, D }) || K->rank != 3 || !is(K, { K->shape[0], hkv, D }) || K->shape[0] < 0 ||
+        !is(V, { K->shape[0], hkv, D }) || T > most || K->shape[0] > most)
+        return RAD_E_SHAPE;
+    if (CQ->rank != 1 || CQ->shape[0] < 1 || CQ->shape[0] > 1 << 24 || (CK && !is(CK, { CQ->shape[0] }))) return RAD_E_SHAPE;
+    if (!word_rows(Q) || !word_rows(K) || !word_rows(V) || !word_rows(O) || !packed(CQ) || (CK && !packed(CK))) return RAD_E_STRIDE;
+    for (const RadTensor* t : { Q, K, V })
+        for (int i = 0; i < 2; ++i)
+            if (t->shape[i] > 1 && (t->stride[i] <= 0 || t->stride[i] >= 1LL << 39)) return RAD_E_STRIDE;
+    g->q = (const uint16_t*)Q->data;
+    g->q_row = Q->stride[0];
+    g->q_head = Q->stride[1];
+    g->k = (const uint16_t*)K->data;
+    g->k_row = K->stride[0];
+    g->k_head = K->stride[1];
+    g->v = (const uint16_t*)V->data;
+    g->v_row = V->stride[0];
+    g->v_head = V->stride[1];
+    g->cu_q = (const int32_t*)CQ->data;
+    g->cu_k = CK ? (const int32_t*)CK->data : g->cu_q;
+    g->o = (uint16_t*)O->data;
+    g->o_row = O->stride[0];
+    g->o_head = O->stride[1];
+    g->T = T;
+    g->Tk = K->shape[0];
+    g->n_seq = CQ->shape[0] - 1;
+    g->n_head = h;
+    g->n_head_kv = hkv;
+    g->head_dim = D;
+    return RAD_OK;
+}
+
 /* ridgefill_attn_decode: q and o bf16 [B, Hq, 256], cache bf16 [2, slots, Hkv, 256] (all read in 16-byte words: dense
  * head rows, bases and other strides multiples of 16 bytes), block_table i32 [B, n_pages] (any row pitch), kv_lens i32
  * [B] dense. Hq a multiple of Hkv, at most 128 query heads a kv head. */
@@ -139,7 +214,7 @@ extern "C" int ridgefill_attn_decode_parse(const RadArgs* a, RidgeFillAttnDecode
         !rad_args_geti(a, "n_head_kv", &hkv) || !rad_args_geti(a, "head_dim", &D) || !rad_args_geti(a, "page", &page))
         return RAD_E_INVAL;
     if (D != 256) return RAD_E_UNSUPPORTED;
-    if (!scale_of(a, D, &g->scale)) return RAD_E_INVAL;
+    if (!scale_of(a, D, true, &g->scale)) return RAD_E_INVAL;
     if (Q->dtype != RAD_BF16 || C->dtype != RAD_BF16 || T->dtype != RAD_I32 || L->dtype != RAD_I32 || O->dtype != RAD_BF16)
         return RAD_E_DTYPE;
     if (B < 0 || h <= 0 || hkv <= 0 || page <= 0 || page > 1 << 20) return RAD_E_SHAPE;
@@ -193,7 +268,7 @@ extern "C" int ridgefill_gdn_step_parse(const RadArgs* a, RidgeFillGdnStep* g) {
         return RAD_E_INVAL;
     const bool wide = dk == 128 && dv == 128, small = dk >= 8 && dk <= 64 && dk % 8 == 0 && dv >= 1 && dv <= 64;
     if (hk <= 0 || hv <= 0 || hv % hk != 0 || !(wide || small)) return RAD_E_UNSUPPORTED;
-    if (!scale_of(a, dk, &g->scale)) return RAD_E_INVAL;
+    if (!scale_of(a, dk, false, &g->scale)) return RAD_E_INVAL;
     if (Q->dtype != RAD_BF16 || K->dtype != RAD_BF16 || V->dtype != RAD_BF16 || G->dtype != RAD_F32 ||
         Be->dtype != RAD_F32 || S->dtype != RAD_F32 || O->dtype != RAD_BF16)
         return RAD_E_DTYPE;

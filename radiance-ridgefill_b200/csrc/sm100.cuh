@@ -34,6 +34,8 @@ static inline int read_device_error(int reset) {
 /* The DeltaNet fill's copy (gdn.cu). */
 int gdn_device_error(int reset);
 int peer_device_error(int reset);
+/* The prompt attention's (attn_prefill.cu). */
+int attn_device_error(int reset);
 
 enum DeviceError : int {
     kErrNone = 0,
@@ -42,6 +44,7 @@ enum DeviceError : int {
     kErrGemmWaitEpilogue = 0x103,
     kErrGemmDrain = 0x104,
     kErrGdnWait = 0x201,
+    kErrAttnWait = 0x401,
 };
 
 constexpr uint64_t kWaitTimeoutNs = 2000000000ull;   /* 2 s */

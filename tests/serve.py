@@ -98,3 +98,29 @@ def step_reference(torch, q, k, v, g, beta, state, idx, out_idx, scale=None):
     do = scale * (U32 * (dk + 16) * torch.einsum("bhvk,bhk->bhv", S.abs(), qq.abs()) + du * kq.abs() +
                   U32 * (dk + 8) * u.abs() * kqm)
     return o, new, 1.01 * UB16 * o.abs() + 2 * do + 1e-30, dS + 1e-35
+
+
+def prefill_params(T, hq, hkv, D=256, scale=None):
+    p = [H.pint("M", T), H.pint("n_head", hq), H.pint("n_head_kv", hkv), H.pint("head_dim", D)]
+    return p + ([H.pf64("scale", scale)] if scale is not None else [])
+
+
+def prefill_reference(torch, q, k, v, cu_q, cu_k, scale=None, heads=None):
+    """(o, bound, written rows) f64 of ridgefill_attn_prefill's formula for in-order cu lists; `heads`: only these."""
+    T, hq, D = q.shape
+    hkv = k.shape[1]
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    o = torch.zeros(T, hq, D, dtype=torch.float64, device=q.device)
+    bound = torch.zeros_like(o)
+    rows = torch.zeros(T, dtype=torch.bool, device=q.device)
+    for q0, q1, k0, k1 in zip(cu_q[:-1], cu_q[1:], cu_k[:-1], cu_k[1:]):
+        nq, nk = q1 - q0, k1 - k0
+        rows[q0:q1] = True
+        keep = torch.ones(nq, nk, dtype=torch.bool, device=q.device).tril(nk - nq)
+        for h in range(hq) if heads is None else heads:
+            qq, kk, vv = q[q0:q1, h].double(), k[k0:k1, h // (hq // hkv)].double(), v[k0:k1, h // (hq // hkv)].double()
+            out, p = attention(torch, qq, kk, vv, scale, keep)
+            o[q0:q1, h] = out
+            # a weight rounded to bf16, and the approximate exponential's 2^-22
+            bound[q0:q1, h] = attention_bound(torch, qq, kk, vv, p, out, scale, 1.01 * UB16)
+    return o, bound, rows

@@ -1,0 +1,214 @@
+"""ridgefill_attn_prefill on B200 against its formula in 64 bits, element by element within the bound of its arithmetic:
+rows and keys around the 128-key tiles and the query tiles, tails, rows without keys, empty and many sequences, every
+kind of head group, strides, rows behind the last sequence, NaN in other sequences and behind them, offsets past 32
+bits; and with the rows it is used with."""
+import pytest
+
+import harness as H
+import serve as S
+from harness import abi
+
+pytestmark = pytest.mark.gpu
+D = 256
+
+
+def ends(lens):
+    out = [0]
+    for n in lens:
+        out.append(out[-1] + n)
+    return out
+
+
+def inputs(torch, seed, nq, nk, hq, hkv, pad=0, gain=2.0):
+    """Packed sequences, `pad` rows behind the last one (q: anything; k, v: NaN)."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, device="cuda", generator=g)   # noqa: E731
+    q = (gain * rn(sum(nq) + pad, hq, D)).to(torch.bfloat16)
+    k, v = (rn(sum(nk) + pad, hkv, D).to(torch.bfloat16) for _ in range(2))
+    k[sum(nk):] = float("nan")
+    v[sum(nk):] = float("nan")
+    return dict(q=q, k=k, v=v, cu_q=ends(nq), cu_k=ends(nk), o=torch.full_like(q, 7.0))
+
+
+def operands(torch, d):
+    cu = [torch.tensor(d[n], dtype=torch.int32, device="cuda") for n in ("cu_q", "cu_k")]
+    same = d["cu_q"] == d["cu_k"]
+    return [H.dev(d["q"]), H.dev(d["k"]), H.dev(d["v"]), H.dev(cu[0]), H.dev(None if same else cu[1]), H.dev(d["o"])], cu
+
+
+def call(lib, torch, d, scale=None):
+    ops, keep = operands(torch, d)
+    T, hq, _ = d["q"].shape
+    rc = H.launch(lib, "ridgefill_attn_prefill", ops, S.prefill_params(T, hq, d["k"].shape[1], scale=scale))
+    assert lib.lib.ridgefill_device_error(1) == 0
+    return rc
+
+
+def check(torch, d, scale=None, heads=None):
+    o, bound, rows = S.prefill_reference(torch, d["q"], d["k"], d["v"], d["cu_q"], d["cu_k"], scale, heads)
+    pick = slice(None) if heads is None else heads
+    err = (d["o"].double() - o).abs()[rows][:, pick]
+    bad = ~(err <= bound[rows][:, pick])
+    assert not bad.any(), f"{int(bad.sum())} elements off, first at {bad.nonzero()[0].tolist()}, {float(err[bad][0])}"
+    assert (d["o"][~rows] == 7.0).all(), "a row outside every sequence was written"
+
+
+@pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 31, 100, 127, 128, 129, 255, 256, 257, 700])
+def test_one_prompt(cuda, product_lib, n):
+    torch = cuda
+    d = inputs(torch, n, [n], [n], 16, 2, pad=n % 3)
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, d)
+
+
+@pytest.mark.parametrize("nq,nk", [(1, 128), (1, 129), (1, 1000), (5, 384), (16, 2000), (40, 4100), (200, 257), (128, 1152)])
+def test_tails(cuda, product_lib, nq, nk):
+    torch = cuda
+    d = inputs(torch, nq + nk, [nq], [nk], 16, 2)
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, d)
+
+
+@pytest.mark.parametrize("nq,nk", [(10, 0), (300, 100), (129, 128), (1, 0), (50, 1)])
+def test_rows_without_keys(cuda, product_lib, nq, nk):
+    """More rows than keys: the first nq - nk rows see none and are zero."""
+    torch = cuda
+    d = inputs(torch, 7 * nq + nk, [nq, 20], [nk, 20], 8, 1)
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, d)
+    assert (d["o"][:nq - nk] == 0).all()
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (2, 2), (4, 1), (12, 2), (9, 3), (16, 1), (20, 1), (48, 3), (100, 1), (128, 1), (130, 2)])
+def test_head_groups(cuda, product_lib, hq, hkv):
+    torch = cuda
+    d = inputs(torch, hq * 10 + hkv, [150, 33], [150, 290], hq, hkv, pad=2)
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, d)
+
+
+@pytest.mark.parametrize("nq", [[300, 0, 45, 128, 1], [0, 0, 7], [17] * 32, [5, 0, 130] * 13, [3] * 100, [0] * 40 + [200] + [0] * 30])
+def test_packed_sequences(cuda, product_lib, nq):
+    """Up to 32 sequences (sorted) and more, empty ones among them; some with more keys than rows."""
+    torch = cuda
+    nk = [n + (37 * i) % 200 if i % 3 == 0 and n else n for i, n in enumerate(nq)]
+    d = inputs(torch, len(nq), nq, nk, 16, 2, pad=5)
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, d)
+
+
+def test_long_prompt(cuda, product_lib):
+    """Many query tiles a CTA, the ring and every barrier through many phases."""
+    torch = cuda
+    d = inputs(torch, 51, [6000, 1500], [6000, 3333], 16, 2)
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, d, heads=[0, 7, 8, 13])
+
+
+def test_weights_far_apart(cuda, product_lib):
+    """Scores that span hundreds, and a maximum that rises along the keys: the sums are rescaled again and again."""
+    torch = cuda
+    d = inputs(torch, 52, [900], [900], 16, 2, gain=40.0)
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, d)
+    d = inputs(torch, 53, [64], [1500], 8, 1)
+    d["q"][:] = d["q"][0, 0]
+    d["k"][:, 0] = (d["q"][0, 0].float()[None] * (torch.arange(1500, device="cuda")[:, None] / 300.0)).to(torch.bfloat16)
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, d)
+    d["k"] = d["k"].flip(0).contiguous()       # and one that falls
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, d)
+
+
+def test_strides_and_scale(cuda, product_lib):
+    """q, k, v slices of one fused projection row, o into a wider row, a scale of its own; k and v as planes of a
+    [rows, 2, Hkv, D] cache."""
+    torch = cuda
+    d = inputs(torch, 54, [140, 60], [140, 60], 12, 2)
+    row = torch.full((200, 16 * D + 8), float("nan"), dtype=torch.bfloat16, device="cuda")
+    for name, at, h in (("q", 0, 12), ("k", 12 * D, 2), ("v", 14 * D, 2)):
+        row[:, at:at + h * D] = d[name].reshape(200, -1)
+        d[name] = row[:, at:at + h * D].view(200, h, D)
+    whole = torch.full((200, 13, D + 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    d["o"] = whole[:, 1:, 8:]
+    assert call(product_lib, torch, d, scale=0.02) == abi.OK
+    check(torch, d, 0.02)
+    whole[:, 1:, 8:] = 7.0
+    assert (whole == 7.0).all()
+    d = inputs(torch, 55, [90], [300], 8, 2)
+    cache = torch.stack([d["k"], d["v"]], 1)
+    d["k"], d["v"] = cache[:, 0], cache[:, 1]
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, d)
+
+
+def test_nan_stays_in_its_sequence(cuda, product_lib):
+    """NaN and infinities in one sequence's q, k and v reach no row of another, nor rows 128 or more before them; keys'
+    NaN reach no earlier row at all."""
+    torch = cuda
+    nq = [100, 200, 70]
+    d = inputs(torch, 56, nq, nq, 16, 2)
+    d["q"][150], d["k"][160], d["v"][299] = float("nan"), float("inf"), float("nan")
+    assert call(product_lib, torch, d) == abi.OK
+    got = d["o"]
+    clean = inputs(torch, 56, nq, nq, 16, 2)
+    assert call(product_lib, torch, clean) == abi.OK
+    same = (got == clean["o"]).all(dim=2).all(dim=1)
+    assert same[:100].all() and same[300:].all() and same[100:150].all()
+    assert torch.isnan(got[150]).all() and torch.isnan(got[299]).all()
+    check(torch, clean)
+
+
+def test_more_than_32_bits_of_keys(cuda, product_lib):
+    """Keys and values at the far end of operands of more than 2^31 elements."""
+    torch = cuda
+    rows, n = 4_300_000, 200
+    k, v = (torch.empty(rows, 2, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    assert k.numel() > 2 ** 31
+    d = inputs(torch, 57, [n], [n], 16, 2)
+    k[-n:], v[-n:] = d["k"], d["v"]
+    small = dict(d)
+    d["k"], d["v"], d["cu_k"] = k, v, [rows - n, rows]
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, dict(small, o=d["o"]))
+
+
+def test_lists_out_of_order(cuda, product_lib):
+    """cu lists outside their operands are clamped, a falling pair is an empty sequence: nothing out of range is read
+    or written."""
+    torch = cuda
+    d = inputs(torch, 58, [60], [60], 8, 2, pad=4)
+    d["cu_q"], d["cu_k"] = [-5, 40, 30, 1 << 30], [-7, 40, 35, 1 << 30]
+    assert call(product_lib, torch, d) == abi.OK
+    k = dict(d, k=torch.nan_to_num(d["k"]), v=torch.nan_to_num(d["v"]))
+    o, bound, rows = S.prefill_reference(torch, k["q"], k["k"], k["v"], [0, 40], [0, 40])
+    assert ((d["o"][:30].double() - o[:30]).abs() <= bound[:30]).all()
+
+
+def test_repeats_streams_and_graphs(cuda, product_lib):
+    """The same call gives the same bits, eagerly and from graphs of two calls replayed side by side."""
+    torch = cuda
+    row = product_lib.find_row("ridgefill_attn_prefill", abi.DOMAIN_DEVICE)
+    calls = []
+    for seed, n in ((59, [500, 33]), (60, [1200])):
+        d = inputs(torch, seed, n, n, 16, 2)
+        assert call(product_lib, torch, d) == abi.OK
+        check(torch, d)
+        ops, keep = operands(torch, d)
+        bound = product_lib.bind(row, ops, S.prefill_params(sum(n), 16, 2))
+        graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(graph, stream=stream):
+            assert bound(torch.cuda.current_stream().cuda_stream) == abi.OK
+        calls.append((d, d["o"].clone(), graph, stream, keep))
+    for _ in range(5):
+        for d, *_ in calls:
+            d["o"].zero_()
+        torch.cuda.synchronize()
+        for _, _, graph, stream, _ in calls:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for d, want, *_ in calls:
+            assert torch.equal(d["o"], want)
+    assert product_lib.lib.ridgefill_device_error(1) == 0

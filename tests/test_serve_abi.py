@@ -10,6 +10,8 @@ import serve as S
 from harness import abi
 
 OPS = {
+    "ridgefill_attn_prefill": (["M", "n_head", "n_head_kv", "head_dim", "scale"],
+                               ["q", "k", "v", "cu_seqlens", "cu_keys", "o"]),
     "ridgefill_attn_decode": (["M", "n_head", "n_head_kv", "head_dim", "page", "scale"],
                               ["q", "kv_cache", "block_table", "kv_lens", "o"]),
     "ridgefill_gdn_step": (["M", "n_head_k", "n_head_v", "head_k", "head_v", "scale"],
@@ -18,7 +20,8 @@ OPS = {
 
 
 def cold_params(op):
-    return {"ridgefill_attn_decode": lambda: S.decode_params(3, 16, 2, 16),
+    return {"ridgefill_attn_prefill": lambda: S.prefill_params(40, 16, 2),
+            "ridgefill_attn_decode": lambda: S.decode_params(3, 16, 2, 16),
             "ridgefill_gdn_step": lambda: S.step_params(3, 2, 4)}[op]()
 
 
@@ -67,6 +70,11 @@ def T(dtype, shape, strides=None, off=0):
     return abi.tensor(dtype, shape, BASE + off, strides)
 
 
+def prefill_case(T_=40, keys=70, hq=16, hkv=2, D=256, n=3):
+    return dict(q=T(abi.BF16, [T_, hq, D]), k=T(abi.BF16, [keys, hkv, D]), v=T(abi.BF16, [keys, hkv, D]),
+                cu_q=T(abi.I32, [n + 1]), cu_k=T(abi.I32, [n + 1]), o=T(abi.BF16, [T_, hq, D]))
+
+
 def decode_case(B=3, hq=16, hkv=2, D=256, page=16, pages=5, slots=400):
     return dict(q=T(abi.BF16, [B, hq, D]), kv_cache=T(abi.BF16, [2, slots, hkv, D]), block_table=T(abi.I32, [B, pages]),
                 kv_lens=T(abi.I32, [B]), o=T(abi.BF16, [B, hq, D]))
@@ -78,6 +86,35 @@ def step_case(B=3, hk=2, hv=4, dk=128, dv=128, slots=5):
                 out_idx=abi.absent(), o=T(abi.BF16, [B, hv, dv]))
 
 
+PREFILL = [
+    (abi.OK, {}, {}),
+    (abi.OK, dict(cu_k=abi.absent()), {}),
+    (abi.OK, dict(q=T(abi.BF16, [40, 16, 256], [20 * 256, 256, 1])), {}),
+    (abi.OK, dict(k=T(abi.BF16, [70, 2, 256], [1024, 256, 1]), v=T(abi.BF16, [70, 2, 256], [1024, 256, 1], off=1024)), {}),
+    (abi.E_INVAL, dict(v=abi.absent()), {}),
+    (abi.E_INVAL, {}, dict(n_head_kv=None)),
+    (abi.E_INVAL, {}, dict(scale=float("nan"))),
+    (abi.E_INVAL, {}, dict(scale=0.0)),
+    (abi.E_INVAL, {}, dict(scale=-0.1)),
+    (abi.E_UNSUPPORTED, {}, dict(head_dim=64)),
+    (abi.E_UNSUPPORTED, {}, dict(n_head_kv=5)),
+    (abi.E_UNSUPPORTED, dict(q=T(abi.BF16, [40, 258, 256])), dict(n_head=258)),                # 129 heads a kv head
+    (abi.E_DTYPE, dict(k=T(abi.F16, [70, 2, 256])), {}),
+    (abi.E_DTYPE, dict(cu_q=T(abi.I64, [4])), {}),
+    (abi.E_DTYPE, dict(o=T(abi.F32, [40, 16, 256])), {}),
+    (abi.E_SHAPE, {}, dict(M=41)),
+    (abi.E_SHAPE, dict(v=T(abi.BF16, [71, 2, 256])), {}),
+    (abi.E_SHAPE, dict(cu_k=T(abi.I32, [3])), {}),
+    (abi.E_SHAPE, dict(cu_q=T(abi.I32, [0])), {}),
+    (abi.E_SHAPE, dict(o=T(abi.BF16, [40, 16, 128])), {}),
+    (abi.E_SHAPE, dict(k=T(abi.BF16, [1 << 31, 2, 256]), v=T(abi.BF16, [1 << 31, 2, 256])), {}),
+    (abi.E_STRIDE, dict(cu_q=T(abi.I32, [4], [2])), {}),
+    (abi.E_STRIDE, dict(q=T(abi.BF16, [40, 16, 256], off=4)), {}),
+    (abi.E_STRIDE, dict(k=T(abi.BF16, [70, 2, 256], [516, 256, 1])), {}),
+    (abi.E_STRIDE, dict(v=T(abi.BF16, [70, 2, 256], [0, 256, 1])), {}),
+    (abi.E_STRIDE, dict(k=T(abi.BF16, [70, 2, 256], [-512, 256, 1])), {}),
+]
+
 DECODE = [
     (abi.OK, {}, {}),
     (abi.OK, dict(block_table=T(abi.I32, [3, 5], [9, 1])), {}),
@@ -87,6 +124,7 @@ DECODE = [
     (abi.E_INVAL, {}, dict(page=None)),
     (abi.E_INVAL, {}, dict(scale=float("nan"))),
     (abi.E_INVAL, {}, dict(scale=float("inf"))),
+    (abi.E_INVAL, {}, dict(scale=-1.0)),
     (abi.E_UNSUPPORTED, {}, dict(head_dim=128)),
     (abi.E_UNSUPPORTED, {}, dict(n_head_kv=3)),                                            # 16 heads over 3
     (abi.E_DTYPE, dict(q=T(abi.F16, [3, 16, 256])), {}),
@@ -145,6 +183,13 @@ def _params(base, change):
     return out + [H.pf64("scale", change["scale"]) for _ in range("scale" in change)]
 
 
+@pytest.mark.parametrize("case", range(len(PREFILL)))
+def test_prefill_refusals(product_lib, case):
+    want, operands, params = PREFILL[case]
+    tensors = list((prefill_case() | operands).values())
+    assert S.parse(product_lib, "ridgefill_attn_prefill_parse", tensors, _params(S.prefill_params(40, 16, 2), params)) == want
+
+
 @pytest.mark.parametrize("case", range(len(DECODE)))
 def test_decode_refusals(product_lib, case):
     want, operands, params = DECODE[case]
@@ -166,6 +211,9 @@ def test_null_arguments(product_lib):
 
 def test_no_rows_is_no_work(product_lib):
     """M = 0 with every operand given: accepted, nothing is launched (so it needs no device)."""
+    row = product_lib.find_row("ridgefill_attn_prefill", abi.DOMAIN_DEVICE)
+    assert product_lib.launch(row, list(prefill_case(T_=0).values()), S.prefill_params(0, 16, 2)) == abi.OK
+    assert product_lib.launch(row, list(prefill_case(n=0).values()), S.prefill_params(40, 16, 2)) == abi.OK
     row = product_lib.find_row("ridgefill_attn_decode", abi.DOMAIN_DEVICE)
     assert product_lib.launch(row, list(decode_case(B=0).values()), S.decode_params(0, 16, 2, 16)) == abi.OK
     row = product_lib.find_row("ridgefill_gdn_step", abi.DOMAIN_DEVICE)

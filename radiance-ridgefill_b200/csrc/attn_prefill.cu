@@ -1,27 +1,30 @@
 /* attn_prefill.cu -- ridgefill_attn_prefill: causal attention of packed prompts on B200 (ridgefill_serve.h holds the
  * formula): the exact rows of a prompt (all of them, or the tail) over its keys, grouped heads, head dim 256.
  *
- * Tensor-bound: 4 D flops a (row, key) pair and query head. S = Q K^T and O = P V run on tcgen05, 128 x 128 x 256 and
- * 128 x 256 x 128 a key tile, each 1,024 cycles at the full rate; the exponentials, 16,384 a tile at 16 a cycle, take
- * another pipe 1,024 cycles beside them.
+ * Tensor-bound: 4 D flops a (row, key) pair and query head. S = Q K^T and O = P V run on tcgen05 over CTA pairs
+ * (cta_group::2): 256 rows x 128 keys x 256 and 256 x 256 x 128 a key tile, 2,048 cycles at the full rate together. The
+ * pair halves what each SM's shared memory carries: one CTA alone would read 192 KiB of operands and take in 128 KiB of
+ * copies a key tile, 2,500 cycles of its 128 bytes a cycle; a CTA of a pair reads 128 KiB and takes in 64 KiB. The
+ * exponentials, 16,384 a CTA and tile at 16 a cycle, take another pipe 1,024 cycles beside them.
  *
- * A query tile is the 128 / group tokens whose rows of all `group` query heads of one kv head fill M = 128, so a key
- * tile is read once for the whole group, and the causal edge cuts at 128 / group rows, not at 128. One persistent CTA a
- * SM takes query tiles from the longest to the shortest, in turns that run back and forth, so that the CTAs' sums are
- * near alike.
+ * A CTA's 128 rows are the 128 / group tokens' rows of all `group` query heads of one kv head, the pair's second CTA
+ * taking the next tokens: a key tile is read once for the whole group, and the causal edge cuts at 2 x 128 / group rows,
+ * not at 256. Persistent pairs take query tiles from the longest to the shortest, in turns that run back and forth, so
+ * that their sums are near alike.
  *
- * Tensor memory (512 columns): two 128-column buffers of scores, and O's 256. P, rounded to bf16, replaces its scores in
- * place (64 columns) and is the second product's A operand from there. Shared memory: Q's 64 KiB and a ring of five
- * 32 KiB stages, a key tile being two stages of K (128 keys x 128 elements) and two of V (64 keys x 256 elements).
- * The issue order S(0), S(1), PV(0), S(2), PV(1), ... gives the softmax of tile j the time of PV(j - 1) and S(j + 1).
- *   warps 0-3   softmax, a thread a row: its 128 scores from tensor memory in one go, maximum, exponentials, sum, P.
- *               The running maximum is followed only when a tile exceeds it by 2^8: rescaling O, 256 columns of tensor
- *               memory a row, is then rare, and the weights of a row stay below 2^8
- *   warps 4-7   the output: O from tensor memory, divided by the row's sum, rounded once to bf16, while the next query
- *               tile's products run; and, where a sequence's last key tile is not full, the zeroing of its V rows past
- *               the end (another sequence's rows, or anything behind the last one: P is zero there, but a NaN times
- *               zero is not)
- *   warp 8      TMA loads     warp 9  the products' issue     warp 10  the order of the query tiles
+ * Tensor memory (512 columns a CTA): two 128-column buffers of scores, and O's 256. P, rounded to bf16, replaces its
+ * scores in place (64 columns) and is the second product's A operand from there. Shared memory: Q's 64 KiB and a ring of
+ * 16 KiB stages; a CTA's share of a key tile is two stages of K (its 64 keys x 128 elements) and two of V (64 keys x its
+ * 128 elements). The issue order S(0), S(1), PV(0), S(2), PV(1), ... gives the softmax of tile j the time of PV(j - 1)
+ * and S(j + 1).
+ *   warps 0-7   softmax, two threads a row: 64 scores each from tensor memory, the maxima exchanged in shared memory,
+ *               exponentials, sums, P. The running maximum is followed only when a tile exceeds it by 2^8: rescaling O,
+ *               256 columns of tensor memory a row, is then rare, and the weights of a row stay below 2^8
+ *   warps 8-11  the output: O from tensor memory, divided by the row's sum, rounded once to bf16, turned in shared memory
+ *               so that four lanes write 64 bytes of a row, while the next query tile's products run; and, where a
+ *               sequence's last key tile is not full, the zeroing of its V rows past the end (another sequence's rows, or
+ *               anything behind the last one: P is zero there, but a NaN times zero is not)
+ *   warp 12     TMA loads     warp 13  the products' issue (the pair's first CTA)     warp 14  the order of the tiles
  * P as bf16 costs half a bf16 step a weight, of the order of the output's own rounding; f32 elsewhere.
  */
 #include <cuda_bf16.h>
@@ -32,39 +35,41 @@
 
 namespace {
 
-constexpr int D = 256, kTileM = 128, kTileN = 128;
-constexpr int kStages = 5, kStageBytes = 32768, kQBytes = kTileM * D * 2;
+constexpr int D = 256, kTileM = 128, kTileN = 128;           /* rows of a CTA (the pair's tile has 256); keys */
+constexpr int kStages = 9, kStageBytes = 16384, kQBytes = kTileM * D * 2;
 constexpr int kBoxBytes = 64 * 64 * 2;                       /* one TMA box of K or V: 64 rows x 64 elements */
-constexpr int kSoftWarps = 4, kOutWarps = 4, kWarps = kSoftWarps + kOutWarps + 3, kThreads = 32 * kWarps;
+constexpr int kSoftWarps = 8, kOutWarps = 4, kWarps = kSoftWarps + kOutWarps + 3, kThreads = 32 * kWarps;
+constexpr int kTurnBytes = 32 * 64;                          /* an output warp's 32 rows x 32 elements */
 constexpr int kRing = 4;                                     /* query tiles announced ahead */
 constexpr uint32_t kTmemCols = 512, kColO = 256;
 constexpr float kGrow = 8.0f, kNone = -INFINITY;
-/* kind::f16, D f32 (bit 4), A and B bf16 (bits 7, 10), N >> 3 at 17, M >> 4 at 24; B MN-major bit 16 */
-constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kTileN >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
-constexpr uint32_t kIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
+/* kind::f16 over the pair, D f32 (bit 4), A and B bf16 (bits 7, 10), N >> 3 at 17, M >> 4 at 24; B MN-major bit 16 */
+constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kTileN >> 3) << 17) | ((uint32_t)(2 * kTileM >> 4) << 24);
+constexpr uint32_t kIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(2 * kTileM >> 4) << 24);
 
 struct Plan {
     RidgeFillAttnPrefill g;
-    int group, tokens;      /* query heads a kv head; tokens a query tile (128 / group) */
+    int group, tokens;      /* query heads a kv head; tokens of a CTA's rows (128 / group) */
     float scale_log2;
 };
 
-/* One query tile: `rows` tokens from row q0 of q, keys from row k0 of k and v, `tiles` key tiles; token t sees the
- * sequence's keys 0 .. limit + t, of which there are `keys`. rows < 0: no more query tiles. */
+/* One query tile as a CTA sees it: `rows` tokens of its own from row q0 of q, keys from row k0 of k and v, `tiles` key
+ * tiles (the pair's); its token t sees the sequence's keys 0 .. limit + t, of which there are `keys`. rows < 0: no more. */
 struct Item {
     int q0, rows, k0, keys, tiles, limit, head;
 };
 
 struct Shared {
     Item item[kRing];
-    float sum[2][kTileM];                  /* rows' sums of the two query tiles under way */
+    float top[2][2][kTileM];               /* rows' maxima of a tile's two halves, by the tile's parity */
+    float sum[2][2][kTileM];               /* rows' sums (two halves) of the two query tiles under way */
     uint64_t item_full[kRing], item_empty[kRing];
     uint64_t q_full, q_empty, kv_full[kStages], kv_empty[kStages];
     uint64_t s_full[2], p_full[2], pv_done[2], v_last, v_clean, o_full, o_empty, sum_full, drain;
     uint32_t tmem;
     int abort;
 };
-constexpr int kSmemBytes = 1024 + kQBytes + kStages * kStageBytes + (int)sizeof(Shared);
+constexpr int kSmemBytes = 1024 + kQBytes + kStages * kStageBytes + kOutWarps * kTurnBytes + (int)sizeof(Shared);
 static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -90,15 +95,16 @@ __device__ __forceinline__ Seq sequence(const RidgeFillAttnPrefill& g, int i) {
     s.nk = (int)min(max((int64_t)g.cu_k[i + 1], (int64_t)s.k0), g.Tk) - s.k0;
     return s;
 }
-/* Query tile i of a sequence. */
-__device__ __forceinline__ Item tile_of(const Seq& s, int i, int tokens, int head) {
+/* Query tile i of a sequence (2 `tokens` of them), the share of the pair's CTA `rank`. */
+__device__ __forceinline__ Item tile_of(const Seq& s, int i, int tokens, int head, int rank) {
     Item t;
-    t.rows = min(tokens, s.nq - i * tokens);
-    t.q0 = s.q0 + i * tokens;
+    const int from = i * 2 * tokens, both = min(2 * tokens, s.nq - from);
+    t.rows = min(max(both - rank * tokens, 0), tokens);
+    t.q0 = s.q0 + from + rank * tokens;
     t.k0 = s.k0;
     t.keys = s.nk;
-    t.limit = s.nk - s.nq + i * tokens;
-    const int last = t.limit + t.rows - 1;   /* the last row's last key */
+    t.limit = s.nk - s.nq + from + rank * tokens;
+    const int last = s.nk - s.nq + from + both - 1;   /* the pair's last row's last key */
     t.tiles = last < 0 ? 0 : last / kTileN + 1;
     t.head = head;
     return t;
@@ -132,65 +138,46 @@ __device__ __forceinline__ int lane_holding(int x, int at, int lane, int* before
     return k;
 }
 
-/* Announces this CTA's query tiles in the ring; the whole warp 10. Up to 32 sequences (a lane each) the tiles go from
- * the most key tiles to the fewest over all sequences, in turns back and forth; with more, in the batch's order. */
-__device__ void order_tiles(const Plan& p, Shared& s, int lane) {
+/* Announces this pair's query tiles in the ring of either CTA; the whole warp 14 of both, which reach the same order by
+ * themselves. Up to 32 sequences (a lane each, `mine`) the tiles go from the most key tiles to the fewest over all
+ * sequences, in turns back and forth; with more, in the batch's order. */
+__device__ void order_tiles(const Plan& p, Shared& s, const Seq& mine, int rank, int lane) {
     const RidgeFillAttnPrefill& g = p.g;
-    const int n_seq = (int)g.n_seq, heads = (int)g.n_head_kv, ctas = gridDim.x;
+    const int n_seq = (int)g.n_seq, heads = (int)g.n_head_kv, pairs = (int)rf::cluster_count_x(), pair = (int)rf::cluster_id_x();
+    const int tokens = 2 * p.tokens;   /* of a query tile */
     const bool sorted = n_seq <= 32;
-    Seq mine = {};
-    int most = 0;
-    if (sorted && lane < n_seq) {
-        mine = sequence(g, lane);
-        if (mine.nq > 0) most = mine.nk / kTileN + 1;
-    }
-    if (sorted)
+    int most = mine.nq > 0 ? mine.nk / kTileN + 1 : 0;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const int total = sorted ? warp_sum(deeper(mine, -1, p.tokens)) : 0;
+    for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const int total = warp_sum(deeper(mine, -1, tokens));
     int block = 0, base = 0;   /* unsorted: the block of 32 sequences reached, and the tiles before it */
     for (int k = 0;; ++k) {
-        const int at = sorted && (k & 1) ? k * ctas + ctas - 1 - (int)blockIdx.x : k * ctas + (int)blockIdx.x;
+        const int at = sorted && (k & 1) ? k * pairs + pairs - 1 - pair : k * pairs + pair;
         const int t = at / heads, head = at - t * heads;
-        Item item = {};
-        item.rows = -1;
+        Item own = {};
+        int owner = -1;
         if (sorted) {
             if (t < total) {
                 int lo = 0, hi = most;   /* the least depth with at most t deeper tiles: tile t has that depth */
                 while (lo < hi) {
                     const int mid = (lo + hi) >> 1;
-                    if (warp_sum(deeper(mine, mid, p.tokens)) <= t) hi = mid;
+                    if (warp_sum(deeper(mine, mid, tokens)) <= t) hi = mid;
                     else lo = mid + 1;
                 }
-                const int more = deeper(mine, lo, p.tokens), same = deeper(mine, lo - 1, p.tokens) - more;
+                const int more = deeper(mine, lo, tokens), same = deeper(mine, lo - 1, tokens) - more;
                 const int in = t - warp_sum(more);
                 int before = 0, sum;
-                const int owner = max(lane_holding(same, in, lane, &before, &sum), 0);
-                const int i = deeper(mine, -1, p.tokens) - (more + same) + (in - before);
-                const Item own = tile_of(mine, i, p.tokens, head);
-                item.q0 = __shfl_sync(0xffffffffu, own.q0, owner);
-                item.rows = __shfl_sync(0xffffffffu, own.rows, owner);
-                item.k0 = __shfl_sync(0xffffffffu, own.k0, owner);
-                item.keys = __shfl_sync(0xffffffffu, own.keys, owner);
-                item.tiles = __shfl_sync(0xffffffffu, own.tiles, owner);
-                item.limit = __shfl_sync(0xffffffffu, own.limit, owner);
-                item.head = head;
+                owner = max(lane_holding(same, in, lane, &before, &sum), 0);
+                own = tile_of(mine, deeper(mine, -1, tokens) - (more + same) + (in - before), p.tokens, head, rank);
             }
         } else {
             for (; block < n_seq; block += 32) {
                 Seq q = {};
                 if (block + lane < n_seq) q = sequence(g, block + lane);
                 int before = 0, sum;
-                const int owner = lane_holding(deeper(q, -1, p.tokens), t - base, lane, &before, &sum);
+                owner = lane_holding(deeper(q, -1, tokens), t - base, lane, &before, &sum);
                 if (owner >= 0) {
-                    const Item own = tile_of(q, t - base - before, p.tokens, head);
-                    item.q0 = __shfl_sync(0xffffffffu, own.q0, owner);
-                    item.rows = __shfl_sync(0xffffffffu, own.rows, owner);
-                    item.k0 = __shfl_sync(0xffffffffu, own.k0, owner);
-                    item.keys = __shfl_sync(0xffffffffu, own.keys, owner);
-                    item.tiles = __shfl_sync(0xffffffffu, own.tiles, owner);
-                    item.limit = __shfl_sync(0xffffffffu, own.limit, owner);
-                    item.head = head;
+                    own = tile_of(q, t - base - before, p.tokens, head, rank);
                     break;
                 }
                 base += sum;
@@ -199,11 +186,12 @@ __device__ void order_tiles(const Plan& p, Shared& s, int lane) {
         const int slot = k % kRing;
         if (!rf::mbar_wait(&s.item_empty[slot], ((k / kRing) & 1) ^ 1, &s.abort, rf::kErrAttnWait)) return;
         __syncwarp();
-        if (lane == 0) {
-            s.item[slot] = item;
+        if (owner < 0) own.rows = -1;
+        if (lane == max(owner, 0)) {
+            s.item[slot] = own;
             rf::mbar_arrive(&s.item_full[slot]);
         }
-        if (item.rows < 0) return;
+        if (owner < 0) return;
     }
 }
 
@@ -227,67 +215,68 @@ struct Items {
 
 /* ------------------------------------------------------------------ roles */
 
-__device__ __forceinline__ void load_stage(Shared& s, uint8_t* ring, const CUtensorMap* map, uint32_t& use, int x, int rows, int row,
-                                           int head) {
-    const uint32_t stage = use % kStages;
-    rf::mbar_arrive_expect_tx(&s.kv_full[stage], kStageBytes);
-    uint8_t* dst = ring + stage * kStageBytes;
-#pragma unroll
-    for (int b = 0; b < 4; ++b)   /* K: two 64-element columns of two 64-row boxes; V: four 64-element columns of one */
-        rf::tma_load_3d(dst + b * kBoxBytes, map, &s.kv_full[stage], x + (rows == 128 ? b >> 1 : b) * 64, head,
-                        row + (rows == 128 ? (b & 1) * 64 : 0));
-    ++use;
-}
-
+/* Both CTAs of the pair; the bytes of both complete on the first CTA's barriers. */
 __device__ void produce(const Plan& p, Shared& s, uint8_t* qtile, uint8_t* ring, const CUtensorMap* map_q, const CUtensorMap* map_k,
-                        const CUtensorMap* map_v, int lane) {
+                        const CUtensorMap* map_v, int rank, int lane) {
     Items items{ s };
     uint32_t use = 0, done = 0;   /* stages filled; query tiles with keys */
-    const uint32_t q_bytes = 4u * (uint32_t)(p.group * p.tokens) * 128u;
+    const uint32_t q_bytes = 2u * 4u * (uint32_t)(p.group * p.tokens) * 128u;
     bool ok = true;
     for (;;) {
         const Item it = items.next(lane);
         if (it.rows < 0) break;
         if (it.tiles == 0) continue;
         if (lane == 0 && ok) {
-            auto stage = [&](const CUtensorMap* map, int x, int rows, int row) {
+            /* a stage: 64 rows of two 64-element columns from element x */
+            auto stage = [&](const CUtensorMap* map, int x, int row) {
                 if (ok) ok = rf::mbar_wait(&s.kv_empty[use % kStages], ((use / kStages) & 1) ^ 1, &s.abort, rf::kErrAttnWait);
-                if (ok) load_stage(s, ring, map, use, x, rows, row, it.head);
+                if (!ok) return;
+                const uint32_t st = use % kStages, bar = rf::map_rank(rf::smem_addr(&s.kv_full[st]), 0);
+                if (rank == 0) rf::mbar_arrive_expect_tx(&s.kv_full[st], 2 * kStageBytes);
+                rf::tma_load_3d_pair(ring + st * kStageBytes, map, bar, x, it.head, row);
+                rf::tma_load_3d_pair(ring + st * kStageBytes + kBoxBytes, map, bar, x + 64, it.head, row);
+                ++use;
             };
             ok = rf::mbar_wait(&s.q_empty, (done & 1) ^ 1, &s.abort, rf::kErrAttnWait);
             if (ok) {
-                rf::mbar_arrive_expect_tx(&s.q_full, q_bytes);
+                const uint32_t bar = rf::map_rank(rf::smem_addr(&s.q_full), 0);
+                if (rank == 0) rf::mbar_arrive_expect_tx(&s.q_full, q_bytes);
                 for (int b = 0; b < D / 64; ++b)
-                    rf::tma_load_3d(qtile + b * kTileM * 128, map_q, &s.q_full, b * 64, it.head * p.group, it.q0);
+                    rf::tma_load_3d_pair(qtile + b * kTileM * 128, map_q, bar, b * 64, it.head * p.group, it.q0);
                 ++done;
             }
             for (int j = 0; j <= it.tiles; ++j) {
-                if (j < it.tiles)
-                    for (int h = 0; h < 2; ++h) stage(map_k, h * 128, 128, it.k0 + j * kTileN);
-                if (j > 0)
-                    for (int h = 0; h < 2; ++h) stage(map_v, 0, 64, it.k0 + (j - 1) * kTileN + h * 64);
+                if (j < it.tiles)   /* this CTA's 64 keys of the tile */
+                    for (int h = 0; h < 2; ++h) stage(map_k, h * 128, it.k0 + j * kTileN + rank * 64);
+                if (j > 0)          /* the tile's keys, this CTA's 128 elements */
+                    for (int h = 0; h < 2; ++h) stage(map_v, rank * 128, it.k0 + (j - 1) * kTileN + h * 64);
             }
         }
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
         if (!ok) break;
     }
-    /* every copy has landed before the CTA's shared memory is given up */
+    /* The products have read every stage that this CTA filled (so its copies have landed) before it leaves. */
     if (lane == 0) {
         const uint64_t t0 = rf::global_ns();
         for (uint32_t u = use > kStages ? use - kStages : 0; u < use; ++u)
-            while (!rf::mbar_try_wait(&s.kv_full[u % kStages], (u / kStages) & 1) && rf::global_ns() - t0 < rf::kWaitTimeoutNs) {
+            while (!rf::mbar_try_wait(&s.kv_empty[u % kStages], (u / kStages) & 1) && rf::global_ns() - t0 < rf::kWaitTimeoutNs) {
             }
         if (done)
-            while (!rf::mbar_try_wait(&s.q_full, (done - 1) & 1) && rf::global_ns() - t0 < rf::kWaitTimeoutNs) {
+            while (!rf::mbar_try_wait(&s.q_empty, (done - 1) & 1) && rf::global_ns() - t0 < rf::kWaitTimeoutNs) {
             }
     }
 }
 
+/* The pair's first CTA. Its barriers count both CTAs' arrivals; its commits arrive in both. */
 __device__ void multiply(Shared& s, const uint8_t* qtile, const uint8_t* ring, uint32_t tmem, int lane) {
     Items items{ s };
     uint32_t use = 0, tile = 0, done = 0, partial = 0;   /* stages read; key tiles; query tiles with keys; with a last tile cut short */
     const uint32_t q_addr = rf::smem_addr(qtile), r_addr = rf::smem_addr(ring);
     bool ok = true;
+    auto commit = [&](uint64_t* bar) {
+        rf::mma_commit_pair(rf::smem_addr(bar));
+        rf::mma_commit_pair(rf::map_rank(rf::smem_addr(bar), 1));
+    };
     for (;;) {
         const Item it = items.next(lane);
         if (it.rows < 0) break;
@@ -298,35 +287,33 @@ __device__ void multiply(Shared& s, const uint8_t* qtile, const uint8_t* ring, u
                 rf::tc_fence_after();
                 return r_addr + (use % kStages) * kStageBytes;
             };
-            auto give = [&]() {
-                rf::mma_commit(&s.kv_empty[use % kStages]);
-                ++use;
-            };
             auto scores = [&](uint32_t t) {
                 for (int h = 0; h < 2 && ok; ++h) {
                     const uint32_t k = take();
                     if (!ok) return;
 #pragma unroll
                     for (int kk = 0; kk < 8; ++kk)
-                        rf::umma_f16(tmem + (t & 1) * kTileN,
-                                     rf::sw128_kmajor_desc(q_addr + (2 * h + (kk >> 2)) * kTileM * 128 + (kk & 3) * 32),
-                                     rf::sw128_kmajor_desc(k + (kk >> 2) * 2 * kBoxBytes + (kk & 3) * 32), kIdescS, (h | kk) != 0);
-                    give();
+                        rf::umma_f16_pair(tmem + (t & 1) * kTileN,
+                                          rf::sw128_kmajor_desc(q_addr + (2 * h + (kk >> 2)) * kTileM * 128 + (kk & 3) * 32),
+                                          rf::sw128_kmajor_desc(k + (kk >> 2) * kBoxBytes + (kk & 3) * 32), kIdescS, (h | kk) != 0);
+                    commit(&s.kv_empty[use++ % kStages]);
                 }
-                rf::mma_commit(&s.s_full[t & 1]);
+                commit(&s.s_full[t & 1]);
             };
             if (ok) ok = rf::mbar_wait(&s.q_full, done & 1, &s.abort, rf::kErrAttnWait);
+            rf::tc_fence_after();
             if (ok) scores(tile);
             for (int j = 0; j < it.tiles && ok; ++j, ++tile) {
                 if (j + 1 < it.tiles) scores(tile + 1);
                 if (!ok) break;
-                if (j + 2 == it.tiles || it.tiles == 1) rf::mma_commit(&s.q_empty);   /* Q's last product is issued */
+                if (j + 2 == it.tiles || it.tiles == 1) commit(&s.q_empty);   /* Q's last product is issued */
                 const bool cut = j + 1 == it.tiles && it.tiles * kTileN > it.keys;
-                if (cut) {   /* the last V rows have landed: those past the sequence may be cleared */
+                if (cut) {   /* the last V rows have landed: those past the sequence may be cleared, in both CTAs */
                     for (uint32_t u = use; u < use + 2 && ok; ++u)
                         ok = rf::mbar_wait(&s.kv_full[u % kStages], (u / kStages) & 1, &s.abort, rf::kErrAttnWait);
                     if (!ok) break;
-                    rf::mbar_arrive(&s.v_last);
+                    rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.v_last), 0));
+                    rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.v_last), 1));
                 }
                 if (!(ok = rf::mbar_wait(&s.p_full[tile & 1], (tile >> 1) & 1, &s.abort, rf::kErrAttnWait))) break;
                 if (j == 0 && !(ok = rf::mbar_wait(&s.o_empty, (done & 1) ^ 1, &s.abort, rf::kErrAttnWait))) break;
@@ -337,13 +324,13 @@ __device__ void multiply(Shared& s, const uint8_t* qtile, const uint8_t* ring, u
                     if (!ok) break;
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                        rf::umma_f16_ts(tmem + kColO, tmem + (tile & 1) * kTileN + (h * 4 + kk) * 8,
-                                        rf::sw128_mnmajor_desc(v + kk * 2048, kBoxBytes), kIdescO, (j | h | kk) != 0);
-                    give();
+                        rf::umma_f16_ts_pair(tmem + kColO, tmem + (tile & 1) * kTileN + (h * 4 + kk) * 8,
+                                             rf::sw128_mnmajor_desc(v + kk * 2048, kBoxBytes), kIdescO, (j | h | kk) != 0);
+                    commit(&s.kv_empty[use++ % kStages]);
                 }
                 if (!ok) break;
-                rf::mma_commit(&s.pv_done[tile & 1]);
-                if (j + 1 == it.tiles) rf::mma_commit(&s.o_full);
+                commit(&s.pv_done[tile & 1]);
+                if (j + 1 == it.tiles) commit(&s.o_full);
             }
             ++done;
         }
@@ -351,7 +338,7 @@ __device__ void multiply(Shared& s, const uint8_t* qtile, const uint8_t* ring, u
         if (!ok) break;
     }
     if (lane == 0) {   /* every product has run before tensor memory is given up */
-        rf::mma_commit(&s.drain);
+        rf::mma_commit_pair(rf::smem_addr(&s.drain));
         const uint64_t t0 = rf::global_ns();
         while (!rf::mbar_try_wait(&s.drain, 0) && rf::global_ns() - t0 < rf::kWaitTimeoutNs) {
         }
@@ -362,28 +349,29 @@ __device__ void multiply(Shared& s, const uint8_t* qtile, const uint8_t* ring, u
 __device__ void soften(const Plan& p, Shared& s, uint32_t tmem, int warp, int lane) {
     Items items{ s };
     uint32_t tile = 0, done = 0;
-    const int row = warp * 32 + lane, token = row / p.group;
-    const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
+    const int quarter = warp & 3, half = warp >> 2;   /* 32 rows; 64 keys of the tile */
+    const int row = quarter * 32 + lane, token = row / p.group;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     const float sl2 = p.scale_log2;
     for (;;) {
         const Item it = items.next(lane);
         if (it.rows < 0) return;
         if (it.tiles == 0) continue;
-        const int limit = it.limit + min(token, it.rows - 1);   /* this row's last key */
+        const int limit = it.limit + min(token, max(it.rows - 1, 0));   /* this row's last key */
         float m = kNone, l0 = 0.f, l1 = 0.f;
         for (int j = 0; j < it.tiles; ++j, ++tile) {
             const bool ok = rf::mbar_wait(&s.s_full[tile & 1], (tile >> 1) & 1, &s.abort, rf::kErrAttnWait);
-            if (!__all_sync(0xffffffffu, ok)) return;
+            if (rf::bar_any(1 + quarter, 64, !ok)) return;   /* the two warps of these rows leave together */
             rf::tc_fence_after();
-            const uint32_t at = mine + (tile & 1) * kTileN;
-            uint32_t x[4][32];
+            const uint32_t at = lanes + (tile & 1) * kTileN;
+            uint32_t x[2][32];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) rf::tmem_ld32(at + 32 * c, x[c]);
+            for (int c = 0; c < 2; ++c) rf::tmem_ld32(at + 64 * half + 32 * c, x[c]);
             rf::tmem_ld_wait();
-            if (j * kTileN + kTileN - 1 > it.limit) {   /* the first token does not see all of the tile */
-                const int last = limit - j * kTileN;
+            if (j * kTileN + 64 * half + 63 > it.limit) {   /* the first token does not see all of these keys */
+                const int last = limit - j * kTileN - 64 * half;
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
                         if (32 * c + e > last) x[c][e] = __float_as_uint(kNone);
@@ -391,156 +379,169 @@ __device__ void soften(const Plan& p, Shared& s, uint32_t tmem, int warp, int la
             float top[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                top[c] = __uint_as_float(x[c][0]);
+                top[c] = __uint_as_float(x[c >> 1][16 * (c & 1)]);
 #pragma unroll
-                for (int e = 1; e < 32; ++e) top[c] = fmaxf(top[c], __uint_as_float(x[c][e]));
+                for (int e = 1; e < 16; ++e) top[c] = fmaxf(top[c], __uint_as_float(x[c >> 1][16 * (c & 1) + e]));
             }
-            const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl2;
+            const float own = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            s.top[tile & 1][half][row] = own;
+            rf::bar_sync(1 + quarter, 64);   /* and both warps have read their scores: P may take their place */
+            const float mt = fmaxf(own, s.top[tile & 1][half ^ 1][row]) * sl2;
             const bool grow = mt > m + kGrow;
             if (__any_sync(0xffffffffu, grow)) {
                 const float up = grow ? mt : m, f = m == kNone ? 0.f : exp2_approx(m - up);
                 m = up;
                 l0 *= f;
                 l1 *= f;
-                if (j > 0) {   /* O so far, in the units of the old maximum; these scores came after PV(tile - 2), so that
-                                * the barrier of PV(tile - 1) is at most one phase behind */
+                if (j > 0) {   /* this half of O so far, in the units of the old maximum; these scores came after
+                                * PV(tile - 2), so that the barrier of PV(tile - 1) is at most one phase behind */
                     const bool there = rf::mbar_wait(&s.pv_done[(tile - 1) & 1], ((tile - 1) >> 1) & 1, &s.abort, rf::kErrAttnWait);
-                    if (!__all_sync(0xffffffffu, there)) return;
+                    if (rf::bar_any(1 + quarter, 64, !there)) return;
                     rf::tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
+                    for (int c = 0; c < D / 64; ++c) {
                         uint32_t o[32];
-                        rf::tmem_ld32(mine + kColO + 32 * c, o);
+                        rf::tmem_ld32(lanes + kColO + (D / 2) * half + 32 * c, o);
                         rf::tmem_ld_wait();
 #pragma unroll
                         for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        rf::tmem_st32(mine + kColO + 32 * c, o);
+                        rf::tmem_st32(lanes + kColO + (D / 2) * half + 32 * c, o);
                     }
                 }
             }
             const float base = m == kNone ? 0.f : -m;
+            uint32_t w[32];
 #pragma unroll
-            for (int c = 0; c < 4; c += 2) {
-                uint32_t w[32];
-#pragma unroll
-                for (int e = 0; e < 64; e += 2) {
-                    float a = base, b = base;
-                    rf::fma2_rn(a, b, __uint_as_float(x[c + (e >> 5)][e & 31]), __uint_as_float(x[c + (e >> 5)][(e & 31) + 1]), sl2, sl2);
-                    a = exp2_approx(a);
-                    b = exp2_approx(b);
-                    l0 += a;
-                    l1 += b;
-                    w[e >> 1] = pack(a, b);
-                }
-                rf::tmem_st32(at + 16 * c, w);
+            for (int e = 0; e < 64; e += 2) {
+                float a = base, b = base;
+                rf::fma2_rn(a, b, __uint_as_float(x[e >> 5][e & 31]), __uint_as_float(x[e >> 5][(e & 31) + 1]), sl2, sl2);
+                a = exp2_approx(a);
+                b = exp2_approx(b);
+                rf::add2_rn(l0, l1, a, b);
+                w[e >> 1] = pack(a, b);
             }
+            rf::tmem_st32(at + 32 * half, w);
             /* The row's sum, announced before the last P so that no warp can be a query tile ahead of another here. The
              * buffer's earlier sums were read before O was given back, which the query tile between waited for. */
-            if (j + 1 == it.tiles) s.sum[done & 1][row] = l0 + l1;
+            if (j + 1 == it.tiles) s.sum[done & 1][half][row] = l0 + l1;
             rf::tmem_st_wait();
             rf::tc_fence_before();
             __syncwarp();
             if (lane == 0) {
                 if (j + 1 == it.tiles) rf::mbar_arrive(&s.sum_full);
-                rf::mbar_arrive(&s.p_full[tile & 1]);
+                rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.p_full[tile & 1]), 0));
             }
         }
         ++done;
     }
 }
 
-__device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint32_t tmem, int warp, int lane) {
+__device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, uint32_t tmem, int warp, int lane) {
     const RidgeFillAttnPrefill& g = p.g;
     Items items{ s };
     uint32_t use = 0, done = 0, partial = 0;
-    const int row = warp * 32 + lane, token = row / p.group, head = row - token * p.group;
+    const int row = warp * 32 + lane;
     const uint32_t mine = tmem + kColO + ((uint32_t)(warp * 32) << 16);
     for (;;) {
         const Item it = items.next(lane);
         if (it.rows < 0) return;
-        uint16_t* out = g.o + (int64_t)(it.q0 + token) * g.o_row + (int64_t)(it.head * p.group + head) * g.o_head;
+        const int live = it.rows * p.group;   /* this CTA's rows */
+        auto row_at = [&](int r) {
+            const int token = r / p.group;
+            return g.o + (int64_t)(it.q0 + token) * g.o_row + (int64_t)(it.head * p.group + r - token * p.group) * g.o_head;
+        };
         if (it.tiles == 0) {   /* no row of the tile has a key */
-            if (token < it.rows)
-                for (int c = 0; c < D / 8; ++c) *(uint4*)(out + 8 * c) = make_uint4(0u, 0u, 0u, 0u);
+            for (int r = warp * 32; r < min(warp * 32 + 32, live); ++r) *(uint4*)(row_at(r) + 8 * lane) = make_uint4(0u, 0u, 0u, 0u);
             continue;
         }
         use += 4 * it.tiles;
-        if (it.tiles * kTileN > it.keys) {   /* V rows of the last tile past the sequence: its last two stages, 64 rows each */
-            const uint32_t u = use - 2 + (uint32_t)(row >> 6);
-            bool ok = rf::mbar_wait(&s.v_last, partial++ & 1, &s.abort, rf::kErrAttnWait);   /* they are the ring's newest then */
-            if (ok) ok = rf::mbar_wait(&s.kv_full[u % kStages], (u / kStages) & 1, &s.abort, rf::kErrAttnWait);
+        if (it.tiles * kTileN > it.keys) {   /* V rows of the last tile past the sequence: the last two stages, 64 rows each */
+            const bool ok = rf::mbar_wait(&s.v_last, partial++ & 1, &s.abort, rf::kErrAttnWait);
             if (!__all_sync(0xffffffffu, ok)) return;
             if ((it.tiles - 1) * kTileN + row >= it.keys) {
-                uint8_t* at = ring + (u % kStages) * kStageBytes + (row & 63) * 128;
+                uint8_t* at = ring + ((use - 2 + (uint32_t)(row >> 6)) % kStages) * kStageBytes + (row & 63) * 128;
 #pragma unroll
-                for (int b = 0; b < 4; ++b)
+                for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int c = 0; c < 8; ++c) *(uint4*)(at + b * kBoxBytes + c * 16) = make_uint4(0u, 0u, 0u, 0u);
             }
             rf::fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) rf::mbar_arrive(&s.v_clean);
+            if (lane == 0) rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.v_clean), 0));
         }
         bool ok = rf::mbar_wait(&s.o_full, done & 1, &s.abort, rf::kErrAttnWait);
         if (ok) ok = rf::mbar_wait(&s.sum_full, done & 1, &s.abort, rf::kErrAttnWait);
         if (!__all_sync(0xffffffffu, ok)) return;
         rf::tc_fence_after();
-        const float sum = s.sum[done & 1][row];
+        const float sum = s.sum[done & 1][0][row] + s.sum[done & 1][1][row];
         const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);   /* no key: zeros; a NaN stays one */
+        uint8_t* tile = turn + warp * kTurnBytes;
+        uint16_t* dst[4];   /* this lane's chunk of the four rows it writes */
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dst[i] = row_at(warp * 32 + 8 * i + (lane >> 2)) + 8 * (lane & 3);
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = 0; c < D / 32; ++c) {   /* 32 elements of the 32 rows: 16-byte chunk v of row r at chunk v ^ (r / 2 % 4) */
             uint32_t o[32];
             rf::tmem_ld32(mine + 32 * c, o);
             rf::tmem_ld_wait();
             if (c + 1 == D / 32) {   /* O's last read */
                 rf::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) rf::mbar_arrive(&s.o_empty);
+                if (lane == 0) rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.o_empty), 0));
             }
-            if (token < it.rows) {
 #pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    uint32_t w[4];
+            for (int v = 0; v < 4; ++v) {
+                uint32_t w[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        w[e] = pack(__uint_as_float(o[8 * v + 2 * e]) * inv, __uint_as_float(o[8 * v + 2 * e + 1]) * inv);
-                    *(uint4*)(out + 32 * c + 8 * v) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
+                for (int e = 0; e < 4; ++e)
+                    w[e] = pack(__uint_as_float(o[8 * v + 2 * e]) * inv, __uint_as_float(o[8 * v + 2 * e + 1]) * inv);
+                *(uint4*)(tile + lane * 64 + ((v ^ (lane >> 1 & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = 8 * i + (lane >> 2), v = lane & 3;
+                if (warp * 32 + r < live) *(uint4*)(dst[i] + 32 * c) = *(const uint4*)(tile + r * 64 + ((v ^ (r >> 1 & 3)) << 4));
+            }
+            __syncwarp();   /* read before the next 32 elements take its place */
         }
         ++done;
     }
 }
 
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                const __grid_constant__ CUtensorMap map_v, const Plan p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* qtile = smem;
     uint8_t* ring = smem + kQBytes;
-    Shared& s = *(Shared*)(ring + kStages * kStageBytes);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t* turn = ring + kStages * kStageBytes;
+    Shared& s = *(Shared*)(turn + kOutWarps * kTurnBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)rf::cluster_rank();
+    Seq mine = {};   /* the ordering warp's first loads, before the barriers stand */
+    if (warp == kWarps - 1 && p.g.n_seq <= 32 && lane < p.g.n_seq) mine = sequence(p.g, lane);
     if (threadIdx.x == 0) {
         for (int i = 0; i < kRing; ++i) {
             rf::mbar_init(&s.item_full[i], 1);
-            rf::mbar_init(&s.item_empty[i], kWarps - 1);   /* every warp but the one that orders them */
+            /* every warp but the one that orders them, and in the second CTA the one that would issue the products */
+            rf::mbar_init(&s.item_empty[i], kWarps - 1 - rank);
         }
-        rf::mbar_init(&s.q_full, 1);
-        rf::mbar_init(&s.q_empty, 1);
+        rf::mbar_init(&s.q_full, 1);    /* first CTA's: its producer, both CTAs' bytes */
+        rf::mbar_init(&s.q_empty, 1);   /* each CTA's: the products' commits */
         for (int i = 0; i < kStages; ++i) {
             rf::mbar_init(&s.kv_full[i], 1);
             rf::mbar_init(&s.kv_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             rf::mbar_init(&s.s_full[i], 1);
-            rf::mbar_init(&s.p_full[i], kSoftWarps);
+            rf::mbar_init(&s.p_full[i], 2 * kSoftWarps);   /* first CTA's: both CTAs' warps */
             rf::mbar_init(&s.pv_done[i], 1);
         }
         rf::mbar_init(&s.v_last, 1);
-        rf::mbar_init(&s.v_clean, kOutWarps);
+        rf::mbar_init(&s.v_clean, 2 * kOutWarps);
         rf::mbar_init(&s.o_full, 1);
-        rf::mbar_init(&s.o_empty, kOutWarps);
+        rf::mbar_init(&s.o_empty, 2 * kOutWarps);
         rf::mbar_init(&s.sum_full, kSoftWarps);
         rf::mbar_init(&s.drain, 1);
         s.abort = 0;
@@ -549,19 +550,20 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         rf::tma_prefetch_map(&map_k);
         rf::tma_prefetch_map(&map_v);
     }
-    if (warp == 9) rf::tmem_alloc<kTmemCols>(&s.tmem);
+    if (warp == 13) rf::tmem_alloc_pair<kTmemCols>(&s.tmem);
     rf::tc_fence_before();
-    __syncthreads();
+    rf::cluster_sync_all();   /* both CTAs' barriers are initialised before either signals the other's */
     rf::tc_fence_after();
     const uint32_t tmem = s.tmem;
-    if (warp < 4) soften(p, s, tmem, warp, lane);
-    else if (warp < 8) output(p, s, ring, tmem, warp - 4, lane);
-    else if (warp == 8) produce(p, s, qtile, ring, &map_q, &map_k, &map_v, lane);
-    else if (warp == 9) multiply(s, qtile, ring, tmem, lane);
-    else order_tiles(p, s, lane);
+    if (warp < 8) soften(p, s, tmem, warp, lane);
+    else if (warp < 12) output(p, s, ring, turn, tmem, warp - 8, lane);
+    else if (warp == 12) produce(p, s, qtile, ring, &map_q, &map_k, &map_v, rank, lane);
+    else if (warp == 14) order_tiles(p, s, mine, rank, lane);
+    else if (rank == 0) multiply(s, qtile, ring, tmem, lane);
     rf::tc_fence_before();
-    __syncthreads();
-    if (warp == 9) rf::tmem_free<kTmemCols>(tmem);
+    rf::cluster_sync_all();   /* no product reads the other CTA's memory any more */
+    rf::tc_fence_after();
+    if (warp == 13) rf::tmem_free_pair<kTmemCols>(tmem);
 }
 
 /* Head rows [T, heads, 256] bf16 as a 3-D tensor map read in boxes of 64 elements x `heads_box` heads x `rows_box` rows,
@@ -597,7 +599,7 @@ extern "C" int ridgefill_attn_prefill_device(const RadArgs* a, RadStream s) {
     p.tokens = kTileM / p.group;
     p.scale_log2 = g.scale * 1.4426950408889634f;
     /* query tiles at most: a sequence's last one may be cut short */
-    const int64_t items = (g.T / p.tokens + g.n_seq) * g.n_head_kv;
+    const int64_t items = (g.T / (2 * p.tokens) + g.n_seq) * g.n_head_kv;
     if (items > 0x3fffffffLL) return RAD_E_SHAPE;
     CUtensorMap mq, mk, mv;
     if (!head_map(&mq, g.q, g.T, g.n_head, g.q_row, g.q_head, p.group, p.tokens)) return RAD_E_DEVICE;
@@ -609,7 +611,7 @@ extern "C" int ridgefill_attn_prefill_device(const RadArgs* a, RadStream s) {
         cudaGetLastError();
         return RAD_E_DEVICE;
     }
-    const int64_t sms = rf::sm_count();
-    prefill_kernel<<<(unsigned)(items < sms ? items : sms), kThreads, kSmemBytes, rf::as_stream(s)>>>(mq, mk, mv, p);
+    const int64_t pairs = rf::sm_count() / 2;
+    prefill_kernel<<<2 * (unsigned)(items < pairs ? items : pairs), kThreads, kSmemBytes, rf::as_stream(s)>>>(mq, mk, mv, p);
     return rf::launch_status();
 }

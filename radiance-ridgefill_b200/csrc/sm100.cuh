@@ -323,6 +323,12 @@ __device__ __forceinline__ void mul2_rn(float& d0, float& d1, float x0, float x1
         : "=f"(d0), "=f"(d1) : "f"(x0), "f"(x1), "f"(y0), "f"(y1));
 }
 
+__device__ __forceinline__ void add2_rn(float& a0, float& a1, float x0, float x1) {   /* a += x */
+    asm("{\n .reg .b64 a, x;\n mov.b64 a, {%0, %1};\n mov.b64 x, {%2, %3};\n add.rn.f32x2 a, a, x;\n"
+        " mov.b64 {%0, %1}, a;\n}"
+        : "+f"(a0), "+f"(a1) : "f"(x0), "f"(x1));
+}
+
 /* A relaxed arrive (no release fence) on a barrier of this cluster: for hand-overs whose data needs no
  * ordering through memory -- a tensor-memory buffer whose reads the arriving thread has already waited for
  * (tcgen05.wait::ld), so the arrive only says that the columns may be overwritten. */
@@ -353,6 +359,16 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
         : "memory");
 }
 
+/* 3-D tile load as tma_load_3d whose bytes complete on the mbarrier at shared::cluster address `bar_caddr`, which may be
+ * the pair's other CTA's. One destination CTA. */
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar_caddr, int32_t x, int32_t y,
+                                                 int32_t z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_addr(dst)), "l"((uint64_t)map), "r"(bar_caddr), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
 /* D[tmem] (+)= A[smem] * B[smem]^T over the CTA pair, int8 x int8 -> int32. Rank 0 issues. */
 __device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -370,6 +386,17 @@ __device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t a_desc, 
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+/* D[tmem] (+)= A[tmem] * B[smem]^T over the CTA pair, f16 / bf16 -> f32 (kind::f16); each CTA's rows of A in its own
+ * tensor memory, row m in lane m, two elements a 32-bit column along K. Rank 0 issues. */
+__device__ __forceinline__ void umma_f16_ts_pair(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 

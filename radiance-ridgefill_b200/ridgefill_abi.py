@@ -145,12 +145,15 @@ class Call:
     """One row's call with its argument block built once: `call(stream)` is the launch alone. It keeps the descriptors,
     not the memory they point to."""
 
+    _hook = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_void_p)   # the launch hook on plain addresses: nothing to convert a call
+
     def __init__(self, row: RadKernelInfo, tensors, params, scratch: int | None = None, scratch_bytes: int = 0):
         self._args, self._keep = Plugin.args(tensors, params, scratch, scratch_bytes)
-        self._launch, self._ref = row.launch, C.byref(self._args)
+        self._launch = self._hook(C.cast(row.launch, C.c_void_p).value)
+        self._at = C.addressof(self._args)
 
     def __call__(self, stream: int | None = None) -> int:
-        return self._launch(self._ref, stream)
+        return self._launch(self._at, stream)
 
 
 class Plugin:

@@ -267,81 +267,83 @@ __device__ void produce(const Plan& p, Shared& s, uint8_t* qtile, uint8_t* ring,
     }
 }
 
-/* The pair's first CTA. Its barriers count both CTAs' arrivals; its commits arrive in both. */
+/* The pair's first CTA, the whole warp in step. Its barriers count both CTAs' arrivals; its commits arrive in both. */
 __device__ void multiply(Shared& s, const uint8_t* qtile, const uint8_t* ring, uint32_t tmem, int lane) {
     Items items{ s };
-    uint32_t use = 0, tile = 0, done = 0, partial = 0;   /* stages read; key tiles; query tiles with keys; with a last tile cut short */
+    uint32_t stage = 0, phase = 0;                       /* the ring's next stage */
+    uint32_t tile = 0, done = 0, partial = 0;            /* key tiles; query tiles with keys; with a last tile cut short */
     const uint32_t q_addr = rf::smem_addr(qtile), r_addr = rf::smem_addr(ring);
     bool ok = true;
-    auto commit = [&](uint64_t* bar) {
-        rf::mma_commit_pair(rf::smem_addr(bar));
-        rf::mma_commit_pair(rf::map_rank(rf::smem_addr(bar), 1));
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (ok) ok = __all_sync(0xffffffffu, rf::mbar_wait(bar, parity, &s.abort, rf::kErrAttnWait));
+        return ok;
     };
-    for (;;) {
-        const Item it = items.next(lane);
-        if (it.rows < 0) break;
-        if (it.tiles == 0) continue;
-        if (lane == 0) {
-            auto take = [&]() -> uint32_t {   /* the next stage's address, its copies landed */
-                if (ok) ok = rf::mbar_wait(&s.kv_full[use % kStages], (use / kStages) & 1, &s.abort, rf::kErrAttnWait);
-                rf::tc_fence_after();
-                return r_addr + (use % kStages) * kStageBytes;
-            };
-            auto scores = [&](uint32_t t) {
-                for (int h = 0; h < 2 && ok; ++h) {
-                    const uint32_t k = take();
-                    if (!ok) return;
-#pragma unroll
-                    for (int kk = 0; kk < 8; ++kk)
-                        rf::umma_f16_pair(tmem + (t & 1) * kTileN,
-                                          rf::sw128_kmajor_desc(q_addr + (2 * h + (kk >> 2)) * kTileM * 128 + (kk & 3) * 32),
-                                          rf::sw128_kmajor_desc(k + (kk >> 2) * kBoxBytes + (kk & 3) * 32), kIdescS, (h | kk) != 0);
-                    commit(&s.kv_empty[use++ % kStages]);
-                }
-                commit(&s.s_full[t & 1]);
-            };
-            if (ok) ok = rf::mbar_wait(&s.q_full, done & 1, &s.abort, rf::kErrAttnWait);
+    auto commit = [&](uint64_t* bar) { rf::mma_commit_pair_warp(rf::smem_addr(bar), 3); };
+    auto next = [&]() {
+        if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+        }
+    };
+    auto scores = [&](uint32_t t) {
+        const uint32_t d = tmem + (t & 1) * kTileN;
+        for (int h = 0; h < 2; ++h) {
+            if (!wait(&s.kv_full[stage], phase)) return;
             rf::tc_fence_after();
-            if (ok) scores(tile);
-            for (int j = 0; j < it.tiles && ok; ++j, ++tile) {
-                if (j + 1 < it.tiles) scores(tile + 1);
-                if (!ok) break;
-                if (j + 2 == it.tiles || it.tiles == 1) commit(&s.q_empty);   /* Q's last product is issued */
-                const bool cut = j + 1 == it.tiles && it.tiles * kTileN > it.keys;
-                if (cut) {   /* the last V rows have landed: those past the sequence may be cleared, in both CTAs */
-                    for (uint32_t u = use; u < use + 2 && ok; ++u)
-                        ok = rf::mbar_wait(&s.kv_full[u % kStages], (u / kStages) & 1, &s.abort, rf::kErrAttnWait);
-                    if (!ok) break;
-                    rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.v_last), 0));
-                    rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.v_last), 1));
-                }
-                if (!(ok = rf::mbar_wait(&s.p_full[tile & 1], (tile >> 1) & 1, &s.abort, rf::kErrAttnWait))) break;
-                if (j == 0 && !(ok = rf::mbar_wait(&s.o_empty, (done & 1) ^ 1, &s.abort, rf::kErrAttnWait))) break;
-                if (cut && !(ok = rf::mbar_wait(&s.v_clean, partial++ & 1, &s.abort, rf::kErrAttnWait))) break;
-                rf::tc_fence_after();
-                for (int h = 0; h < 2 && ok; ++h) {
-                    const uint32_t v = take();
-                    if (!ok) break;
+            const uint64_t a = rf::sw128_kmajor_desc(q_addr + 2 * h * kTileM * 128), b = rf::sw128_kmajor_desc(r_addr + stage * kStageBytes);
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        rf::umma_f16_ts_pair(tmem + kColO, tmem + (tile & 1) * kTileN + (h * 4 + kk) * 8,
-                                             rf::sw128_mnmajor_desc(v + kk * 2048, kBoxBytes), kIdescO, (j | h | kk) != 0);
-                    commit(&s.kv_empty[use++ % kStages]);
-                }
-                if (!ok) break;
-                commit(&s.pv_done[tile & 1]);
-                if (j + 1 == it.tiles) commit(&s.o_full);
+            for (int kk = 0; kk < 8; ++kk)   /* descriptors count 16 bytes */
+                rf::umma_f16_pair_warp(d, a + (((kk >> 2) * kTileM * 128 + (kk & 3) * 32) >> 4), b + (((kk >> 2) * kBoxBytes + (kk & 3) * 32) >> 4),
+                                       kIdescS, (h | kk) != 0);
+            commit(&s.kv_empty[stage]);
+            next();
+        }
+        commit(&s.s_full[t & 1]);
+    };
+    while (ok) {
+        const Item it = items.next(lane);
+        const int rows = __shfl_sync(0xffffffffu, it.rows, 0), tiles = __shfl_sync(0xffffffffu, it.tiles, 0);
+        if (rows < 0) break;
+        if (tiles == 0) continue;
+        const bool short_last = __shfl_sync(0xffffffffu, tiles * kTileN > it.keys, 0);
+        if (!wait(&s.q_full, done & 1)) break;
+        scores(tile);
+        for (int j = 0; j < tiles && ok; ++j, ++tile) {
+            if (j + 1 < tiles) scores(tile + 1);
+            if (!ok) break;
+            if (j + 2 == tiles || tiles == 1) commit(&s.q_empty);   /* Q's last product is issued */
+            const bool cut = j + 1 == tiles && short_last;
+            if (cut) {   /* the last V rows have landed: those past the sequence may be cleared, in both CTAs */
+                const uint32_t second = stage + 1 == kStages ? 0 : stage + 1;
+                if (!wait(&s.kv_full[stage], phase) || !wait(&s.kv_full[second], second ? phase : phase ^ 1)) break;
+                if (lane < 2) rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.v_last), lane));
+                __syncwarp();
             }
-            ++done;
+            if (!wait(&s.p_full[tile & 1], (tile >> 1) & 1)) break;
+            if (j == 0 && !wait(&s.o_empty, (done & 1) ^ 1)) break;
+            if (cut && !wait(&s.v_clean, partial++ & 1)) break;
+            rf::tc_fence_after();
+            const uint32_t a = tmem + (tile & 1) * kTileN;
+            for (int h = 0; h < 2; ++h) {
+                if (!wait(&s.kv_full[stage], phase)) break;
+                rf::tc_fence_after();
+                const uint64_t b = rf::sw128_mnmajor_desc(r_addr + stage * kStageBytes, kBoxBytes);
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                    rf::umma_f16_ts_pair_warp(tmem + kColO, a + (h * 4 + kk) * 8, b + (kk * 2048 >> 4), kIdescO, (j | h | kk) != 0);
+                commit(&s.kv_empty[stage]);
+                next();
+            }
+            if (!ok) break;
+            commit(&s.pv_done[tile & 1]);
+            if (j + 1 == tiles) commit(&s.o_full);
         }
-        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-        if (!ok) break;
+        ++done;
     }
-    if (lane == 0) {   /* every product has run before tensor memory is given up */
-        rf::mma_commit_pair(rf::smem_addr(&s.drain));
-        const uint64_t t0 = rf::global_ns();
-        while (!rf::mbar_try_wait(&s.drain, 0) && rf::global_ns() - t0 < rf::kWaitTimeoutNs) {
-        }
+    /* every product has run before tensor memory is given up */
+    rf::mma_commit_pair_warp(rf::smem_addr(&s.drain), 1);
+    const uint64_t t0 = rf::global_ns();
+    while (!rf::mbar_try_wait(&s.drain, 0) && rf::global_ns() - t0 < rf::kWaitTimeoutNs) {
     }
     __syncwarp();
 }

@@ -389,21 +389,42 @@ __device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t a_desc, 
         : "memory");
 }
 
-/* D[tmem] (+)= A[tmem] * B[smem]^T over the CTA pair, f16 / bf16 -> f32 (kind::f16); each CTA's rows of A in its own
- * tensor memory, row m in lane m, two elements a 32-bit column along K. Rank 0 issues. */
-__device__ __forceinline__ void umma_f16_ts_pair(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
 /* Arrive on the mbarrier at shared::cluster address `bar_caddr` (either CTA of the pair) once every pair MMA
  * this thread issued so far has completed. */
 __device__ __forceinline__ void mma_commit_pair(uint32_t bar_caddr) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_caddr) : "memory");
+}
+
+/* The same products and commit issued by a whole converged warp, one elected lane of it doing so: with every lane in step
+ * the descriptors are computed in the warp's uniform registers, where the instruction wants them. From a branch that one
+ * lane takes they are moved there one by one, which bounds the rate of issue (about 150 cycles a product). */
+__device__ __forceinline__ void umma_f16_pair_warp(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+/* A in tensor memory: each CTA's rows in its own, row m in lane m, two elements a 32-bit column along K. */
+__device__ __forceinline__ void umma_f16_ts_pair_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+/* Arrives on the barrier at shared address `bar` in every CTA of the pair whose bit `ctas` has. */
+__device__ __forceinline__ void mma_commit_pair_warp(uint32_t bar, uint16_t ctas) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}\n"
+        ::"r"(bar), "h"(ctas)
+        : "memory");
 }
 
 /* Arrive on `bar` once every tcgen05.mma this thread issued so far has completed. */

@@ -62,10 +62,10 @@ struct Item {
 struct Shared {
     Item item[kRing];
     float top[2][2][kTileM];               /* rows' maxima of a tile's two halves, by the tile's parity */
-    float sum[2][2][kTileM];               /* rows' sums (two halves) of the two query tiles under way */
+    float sum[3][2][kTileM];               /* rows' sums (two halves) of the query tiles under way */
     uint64_t item_full[kRing], item_empty[kRing];
     uint64_t q_full, q_empty, kv_full[kStages], kv_empty[kStages];
-    uint64_t s_full[2], p_full[2], pv_done[2], v_last, v_clean, o_full, o_empty, sum_full, drain;
+    uint64_t s_full[2], p_full[2], pv_done[2], v_last, v_clean, o_full, o_empty, sum_full[3], drain;
     uint32_t tmem;
     int abort;
 };
@@ -267,78 +267,96 @@ __device__ void produce(const Plan& p, Shared& s, uint8_t* qtile, uint8_t* ring,
     }
 }
 
-/* The pair's first CTA, the whole warp in step. Its barriers count both CTAs' arrivals; its commits arrive in both. */
+/* The pair's first CTA, the whole warp in step. Its barriers count both CTAs' arrivals; its commits arrive in both. Each
+ * lane watches a barrier of its own, so that all that a product needs costs one wait. The scores of a query tile's first
+ * key tile are issued before the last PV of the query tile before it, while that one's softmax is under way: K(0) lies
+ * behind V(last) in the ring. */
 __device__ void multiply(Shared& s, const uint8_t* qtile, const uint8_t* ring, uint32_t tmem, int lane) {
     Items items{ s };
-    uint32_t stage = 0, phase = 0;                       /* the ring's next stage */
-    uint32_t tile = 0, done = 0, partial = 0;            /* key tiles; query tiles with keys; with a last tile cut short */
+    uint32_t use = 0;                                    /* the ring's next stage, counted through */
+    uint32_t tile = 0, begun = 0, done = 0, partial = 0;   /* the PV's key tile; query tiles with keys begun, done; with a cut last tile */
     const uint32_t q_addr = rf::smem_addr(qtile), r_addr = rf::smem_addr(ring);
     bool ok = true;
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (ok) ok = __all_sync(0xffffffffu, rf::mbar_wait(bar, parity, &s.abort, rf::kErrAttnWait));
+    /* lane 0 .. 3: a barrier and its parity; the other lanes watch lane 0's */
+    auto wait = [&](uint64_t* b0, uint32_t p0, uint64_t* b1, uint32_t p1, uint64_t* b2, uint32_t p2, uint64_t* b3, uint32_t p3) {
+        uint64_t* bar = lane == 1 ? b1 : lane == 2 ? b2 : lane == 3 ? b3 : b0;
+        const uint32_t parity = lane == 1 ? p1 : lane == 2 ? p2 : lane == 3 ? p3 : p0;
+        if (ok) ok = rf::mbar_wait_lanes(bar, parity, &s.abort, rf::kErrAttnWait);
+        rf::tc_fence_after();
         return ok;
     };
+    auto full = [&](uint32_t u) { return &s.kv_full[u % kStages]; };
+    auto phase = [&](uint32_t u) { return (u / kStages) & 1; };
     auto commit = [&](uint64_t* bar) { rf::mma_commit_pair_warp(rf::smem_addr(bar), 3); };
-    auto next = [&]() {
-        if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1;
+    Item it = {}, ahead = {};   /* the query tiles of the PV and of the scores under way */
+    int j = -1, ja = 0;         /* their key tiles; j -1: no PV yet */
+    for (bool first = true; ok;) {
+        /* the scores' key tile: the next of this query tile, or the first of the next with keys */
+        if (first) {
+            do {
+                const Item i = items.next(lane);
+                ahead.rows = __shfl_sync(0xffffffffu, i.rows, 0);
+                ahead.tiles = __shfl_sync(0xffffffffu, i.tiles, 0);
+                ahead.keys = __shfl_sync(0xffffffffu, i.keys, 0);
+            } while (ahead.rows >= 0 && ahead.tiles == 0);
+            ja = 0;
         }
-    };
-    auto scores = [&](uint32_t t) {
-        const uint32_t d = tmem + (t & 1) * kTileN;
-        for (int h = 0; h < 2; ++h) {
-            if (!wait(&s.kv_full[stage], phase)) return;
-            rf::tc_fence_after();
-            const uint64_t a = rf::sw128_kmajor_desc(q_addr + 2 * h * kTileM * 128), b = rf::sw128_kmajor_desc(r_addr + stage * kStageBytes);
+        const bool more = ahead.rows >= 0;
+        const uint32_t k = j >= 0 && first ? use + 2 : use;       /* K: behind this tile's V when it is a new query tile's */
+        const uint32_t v = j >= 0 && !first ? use + 2 : use;
+        if (more) {
+            uint64_t* q = first ? &s.q_full : full(k);
+            const uint32_t pq = first ? begun & 1 : phase(k);
+            if (!wait(full(k), phase(k), full(k + 1), phase(k + 1), q, pq, q, pq)) break;
+            begun += first;
+            const uint32_t d = tmem + (j >= 0 ? (tile + 1) & 1 : 0) * kTileN;
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk)   /* descriptors count 16 bytes */
-                rf::umma_f16_pair_warp(d, a + (((kk >> 2) * kTileM * 128 + (kk & 3) * 32) >> 4), b + (((kk >> 2) * kBoxBytes + (kk & 3) * 32) >> 4),
-                                       kIdescS, (h | kk) != 0);
-            commit(&s.kv_empty[stage]);
-            next();
+            for (int h = 0; h < 2; ++h) {
+                const uint64_t a = rf::sw128_kmajor_desc(q_addr + 2 * h * kTileM * 128),
+                               b = rf::sw128_kmajor_desc(r_addr + (k + h) % kStages * kStageBytes);
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk)   /* descriptors count 16 bytes */
+                    rf::umma_f16_pair_warp(d, a + (((kk >> 2) * kTileM * 128 + (kk & 3) * 32) >> 4), b + (((kk >> 2) * kBoxBytes + (kk & 3) * 32) >> 4),
+                                           kIdescS, (h | kk) != 0);
+                commit(&s.kv_empty[(k + h) % kStages]);
+            }
+            commit(&s.s_full[j >= 0 ? (tile + 1) & 1 : 0]);
+            if (ja + 1 == ahead.tiles) commit(&s.q_empty);   /* Q's last product is issued */
+            use += 2;
         }
-        commit(&s.s_full[t & 1]);
-    };
-    while (ok) {
-        const Item it = items.next(lane);
-        const int rows = __shfl_sync(0xffffffffu, it.rows, 0), tiles = __shfl_sync(0xffffffffu, it.tiles, 0);
-        if (rows < 0) break;
-        if (tiles == 0) continue;
-        const bool short_last = __shfl_sync(0xffffffffu, tiles * kTileN > it.keys, 0);
-        if (!wait(&s.q_full, done & 1)) break;
-        scores(tile);
-        for (int j = 0; j < tiles && ok; ++j, ++tile) {
-            if (j + 1 < tiles) scores(tile + 1);
-            if (!ok) break;
-            if (j + 2 == tiles || tiles == 1) commit(&s.q_empty);   /* Q's last product is issued */
-            const bool cut = j + 1 == tiles && short_last;
+        if (j >= 0) {
+            const bool last = j + 1 == it.tiles, cut = last && it.tiles * kTileN > it.keys;
             if (cut) {   /* the last V rows have landed: those past the sequence may be cleared, in both CTAs */
-                const uint32_t second = stage + 1 == kStages ? 0 : stage + 1;
-                if (!wait(&s.kv_full[stage], phase) || !wait(&s.kv_full[second], second ? phase : phase ^ 1)) break;
+                if (!wait(full(v), phase(v), full(v + 1), phase(v + 1), full(v), phase(v), full(v), phase(v))) break;
                 if (lane < 2) rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.v_last), lane));
                 __syncwarp();
             }
-            if (!wait(&s.p_full[tile & 1], (tile >> 1) & 1)) break;
-            if (j == 0 && !wait(&s.o_empty, (done & 1) ^ 1)) break;
-            if (cut && !wait(&s.v_clean, partial++ & 1)) break;
-            rf::tc_fence_after();
+            uint64_t* p = &s.p_full[tile & 1];
+            const uint32_t pp = (tile >> 1) & 1;
+            if (!wait(p, pp, full(v), phase(v), full(v + 1), phase(v + 1), j == 0 ? &s.o_empty : p, j == 0 ? (done & 1) ^ 1 : pp)) break;
+            if (cut && !wait(&s.v_clean, partial & 1, &s.v_clean, partial & 1, &s.v_clean, partial & 1, &s.v_clean, partial & 1)) break;
+            partial += cut;
             const uint32_t a = tmem + (tile & 1) * kTileN;
+#pragma unroll
             for (int h = 0; h < 2; ++h) {
-                if (!wait(&s.kv_full[stage], phase)) break;
-                rf::tc_fence_after();
-                const uint64_t b = rf::sw128_mnmajor_desc(r_addr + stage * kStageBytes, kBoxBytes);
+                const uint64_t b = rf::sw128_mnmajor_desc(r_addr + (v + h) % kStages * kStageBytes, kBoxBytes);
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)
                     rf::umma_f16_ts_pair_warp(tmem + kColO, a + (h * 4 + kk) * 8, b + (kk * 2048 >> 4), kIdescO, (j | h | kk) != 0);
-                commit(&s.kv_empty[stage]);
-                next();
+                commit(&s.kv_empty[(v + h) % kStages]);
             }
-            if (!ok) break;
             commit(&s.pv_done[tile & 1]);
-            if (j + 1 == tiles) commit(&s.o_full);
+            if (last) {
+                commit(&s.o_full);
+                ++done;
+            }
+            use += 2;
+            ++tile;
         }
-        ++done;
+        if (!more) break;
+        it = ahead;
+        j = ja;
+        first = ++ja == it.tiles;
     }
     /* every product has run before tensor memory is given up */
     rf::mma_commit_pair_warp(rf::smem_addr(&s.drain), 1);
@@ -350,7 +368,8 @@ __device__ void multiply(Shared& s, const uint8_t* qtile, const uint8_t* ring, u
 
 __device__ void soften(const Plan& p, Shared& s, uint32_t tmem, int warp, int lane) {
     Items items{ s };
-    uint32_t tile = 0, done = 0;
+    uint32_t tile = 0;
+    int buf = 2;   /* of the sums */
     const int quarter = warp & 3, half = warp >> 2;   /* 32 rows; 64 keys of the tile */
     const int row = quarter * 32 + lane, token = row / p.group;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
@@ -361,6 +380,7 @@ __device__ void soften(const Plan& p, Shared& s, uint32_t tmem, int warp, int la
         if (it.tiles == 0) continue;
         const int limit = it.limit + min(token, max(it.rows - 1, 0));   /* this row's last key */
         float m = kNone, l0 = 0.f, l1 = 0.f;
+        buf = buf == 2 ? 0 : buf + 1;
         for (int j = 0; j < it.tiles; ++j, ++tile) {
             const bool ok = rf::mbar_wait(&s.s_full[tile & 1], (tile >> 1) & 1, &s.abort, rf::kErrAttnWait);
             if (rf::bar_any(1 + quarter, 64, !ok)) return;   /* the two warps of these rows leave together */
@@ -423,19 +443,19 @@ __device__ void soften(const Plan& p, Shared& s, uint32_t tmem, int warp, int la
                 w[e >> 1] = pack(a, b);
             }
             rf::tmem_st32(at + 32 * half, w);
-            /* The row's sum, announced before the last P so that no warp can be a query tile ahead of another here. The
-             * buffer's earlier sums were read before O was given back, which the query tile between waited for. */
-            if (j + 1 == it.tiles) s.sum[done & 1][half][row] = l0 + l1;
+            /* The row's sum, announced before the last P so that no warp can be a query tile ahead of another here. Three
+             * buffers: these scores may come before the last PV of the query tile before, but not before that of the one
+             * before it, whose first PV waited for O's reader to be done with the buffer's earlier sums. */
+            if (j + 1 == it.tiles) s.sum[buf][half][row] = l0 + l1;
             rf::tmem_st_wait();
             rf::tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                if (j + 1 == it.tiles) rf::mbar_arrive(&s.sum_full);
+                if (j + 1 == it.tiles) rf::mbar_arrive(&s.sum_full[buf]);
                 /* relaxed: P is ordered by tensor memory's own fences, and a release to the cluster costs 1,800 cycles */
                 rf::mbar_arrive_cluster_relaxed(rf::map_rank(rf::smem_addr(&s.p_full[tile & 1]), 0));
             }
         }
-        ++done;
     }
 }
 
@@ -473,10 +493,10 @@ __device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, u
             if (lane == 0) rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.v_clean), 0));
         }
         bool ok = rf::mbar_wait(&s.o_full, done & 1, &s.abort, rf::kErrAttnWait);
-        if (ok) ok = rf::mbar_wait(&s.sum_full, done & 1, &s.abort, rf::kErrAttnWait);
+        if (ok) ok = rf::mbar_wait(&s.sum_full[done % 3], (done / 3) & 1, &s.abort, rf::kErrAttnWait);
         if (!__all_sync(0xffffffffu, ok)) return;
         rf::tc_fence_after();
-        const float sum = s.sum[done & 1][0][row] + s.sum[done & 1][1][row];
+        const float sum = s.sum[done % 3][0][row] + s.sum[done % 3][1][row];
         const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);   /* no key: zeros; a NaN stays one */
         uint8_t* tile = turn + warp * kTurnBytes;
         uint16_t* dst[4];   /* this lane's chunk of the four rows it writes */
@@ -545,7 +565,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         rf::mbar_init(&s.v_clean, 2 * kOutWarps);
         rf::mbar_init(&s.o_full, 1);
         rf::mbar_init(&s.o_empty, 2 * kOutWarps);
-        rf::mbar_init(&s.sum_full, kSoftWarps);
+        for (int i = 0; i < 3; ++i) rf::mbar_init(&s.sum_full[i], kSoftWarps);
         rf::mbar_init(&s.drain, 1);
         s.abort = 0;
         rf::mbar_init_fence();

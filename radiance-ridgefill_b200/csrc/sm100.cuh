@@ -84,6 +84,38 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
     return done != 0;
 }
 
+/* mbar_try_wait without the hardware's suspension: for lanes that watch different barriers. */
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
+/* A warp's wait for the barriers its lanes name (each its own phase), bounded and recorded as mbar_wait. */
+__device__ __forceinline__ bool mbar_wait_lanes(uint64_t* bar, uint32_t parity, volatile int* abort, int err) {
+    if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
+    const uint64_t t0 = global_ns();
+    for (uint32_t i = 1;; ++i) {
+        if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
+        if ((i & 255) == 0) {
+            const bool late = global_ns() - t0 > kWaitTimeoutNs;
+            if (__any_sync(0xffffffffu, *abort != 0 || late)) {
+                if (late) {
+                    *abort = 1;
+                    atomicCAS(&g_device_error, 0, err);
+                }
+                return false;
+            }
+        }
+    }
+}
+
 /* Wait for the phase of `bar` with parity `parity`; false (and *abort raised, the error recorded)
  * after the timeout, or at once when another role already raised *abort. */
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int err) {

@@ -314,10 +314,7 @@ __device__ void multiply(Shared& s, const uint8_t* qtile, const uint8_t* ring, u
             for (int h = 0; h < 2; ++h) {
                 const uint64_t a = rf::sw128_kmajor_desc(q_addr + 2 * h * kTileM * 128),
                                b = rf::sw128_kmajor_desc(r_addr + (k + h) % kStages * kStageBytes);
-#pragma unroll
-                for (int kk = 0; kk < 8; ++kk)   /* descriptors count 16 bytes */
-                    rf::umma_f16_pair_warp(d, a + (((kk >> 2) * kTileM * 128 + (kk & 3) * 32) >> 4), b + (((kk >> 2) * kBoxBytes + (kk & 3) * 32) >> 4),
-                                           kIdescS, (h | kk) != 0);
+                rf::umma_f16_pair_warp8<kTileM * 128, kBoxBytes>(d, a, b, kIdescS, h);
                 commit(&s.kv_empty[(k + h) % kStages]);
             }
             commit(&s.s_full[j >= 0 ? (tile + 1) & 1 : 0]);
@@ -340,9 +337,7 @@ __device__ void multiply(Shared& s, const uint8_t* qtile, const uint8_t* ring, u
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const uint64_t b = rf::sw128_mnmajor_desc(r_addr + (v + h) % kStages * kStageBytes, kBoxBytes);
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                    rf::umma_f16_ts_pair_warp(tmem + kColO, a + (h * 4 + kk) * 8, b + (kk * 2048 >> 4), kIdescO, (j | h | kk) != 0);
+                rf::umma_f16_ts_pair_warp4(tmem + kColO, a + h * 32, b, kIdescO, j | h);
                 commit(&s.kv_empty[(v + h) % kStages]);
             }
             commit(&s.pv_done[tile & 1]);
@@ -383,7 +378,6 @@ __device__ void soften(const Plan& p, Shared& s, uint32_t tmem, int warp, int la
         buf = buf == 2 ? 0 : buf + 1;
         for (int j = 0; j < it.tiles; ++j, ++tile) {
             const bool ok = rf::mbar_wait(&s.s_full[tile & 1], (tile >> 1) & 1, &s.abort, rf::kErrAttnWait);
-            if (rf::bar_any(1 + quarter, 64, !ok)) return;   /* the two warps of these rows leave together */
             rf::tc_fence_after();
             const uint32_t at = lanes + (tile & 1) * kTileN;
             uint32_t x[2][32];
@@ -407,7 +401,8 @@ __device__ void soften(const Plan& p, Shared& s, uint32_t tmem, int warp, int la
             }
             const float own = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
             s.top[tile & 1][half][row] = own;
-            rf::bar_sync(1 + quarter, 64);   /* and both warps have read their scores: P may take their place */
+            /* both warps have read their scores, so that P may take their place; they leave together when a wait gave up */
+            if (rf::bar_any(1 + quarter, 64, !ok)) return;
             const float mt = fmaxf(own, s.top[tile & 1][half ^ 1][row]) * sl2;
             const bool grow = mt > m + kGrow;
             if (__any_sync(0xffffffffu, grow)) {

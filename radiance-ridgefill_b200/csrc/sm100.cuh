@@ -429,23 +429,37 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t bar_caddr) {
 
 /* The same products and commit issued by a whole converged warp, one elected lane of it doing so: with every lane in step
  * the descriptors are computed in the warp's uniform registers, where the instruction wants them. From a branch that one
- * lane takes they are moved there one by one, which bounds the rate of issue (about 150 cycles a product). */
-__device__ __forceinline__ void umma_f16_pair_warp(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+ * lane takes they are moved there one by one, which bounds the rate of issue (about 150 cycles a product).
+ * umma_f16_pair_warp8: eight products along K, 128 of it: A and B K-major tiles of two 64-element atoms each, `a_atom` and
+ * `b_atom` bytes apart; `accumulate` 0: the first one starts D. */
+template <int a_atom, int b_atom>
+__device__ __forceinline__ void umma_f16_pair_warp8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p, e;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
+        "{\n\t.reg .pred p, t, e;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
         "elect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "add.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, t;\n\t"
+        "add.s64 a, %1, 4;\n\tadd.s64 b, %2, 4;\n\t@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, t;\n\t"
+        "add.s64 a, %1, 6;\n\tadd.s64 b, %2, 6;\n\t@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, t;\n\t"
+        "add.s64 a, %1, %5;\n\tadd.s64 b, %2, %6;\n\t@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, t;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, t;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, t;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, t;\n\t}\n"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "n"(a_atom / 16), "n"(b_atom / 16)
         : "memory");
 }
-/* A in tensor memory: each CTA's rows in its own, row m in lane m, two elements a 32-bit column along K. */
-__device__ __forceinline__ void umma_f16_ts_pair_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+/* Four products along K, 64 of it: A in tensor memory (each CTA's rows in its own, row m in lane m, two elements a 32-bit
+ * column along K), B an MN-major tile (16 of K are 2,048 bytes). */
+__device__ __forceinline__ void umma_f16_ts_pair_warp4(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p, e;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
+        "{\n\t.reg .pred p, t, e;\n\t.reg .b64 b;\n\t.reg .b32 a;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
         "elect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "add.s32 a, %1, 8;\n\tadd.s64 b, %2, 128;\n\t@e tcgen05.mma.cta_group::2.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "add.s32 a, %1, 16;\n\tadd.s64 b, %2, 256;\n\t@e tcgen05.mma.cta_group::2.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "add.s32 a, %1, 24;\n\tadd.s64 b, %2, 384;\n\t@e tcgen05.mma.cta_group::2.kind::f16 [%0], [a], b, %3, t;\n\t}\n"
         ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }

@@ -111,11 +111,11 @@ __device__ __forceinline__ Item tile_of(const Seq& s, int i, int tokens, int hea
 }
 /* How many query tiles of a sequence have more than `depth` key tiles: the last ones. depth -1: all. */
 __device__ __forceinline__ int deeper(const Seq& s, int depth, int tokens) {
-    const int all = (s.nq + tokens - 1) / tokens;
+    const int all = (int)((uint32_t)(s.nq + tokens - 1) / (uint32_t)tokens);
     if (depth < 0) return all;
-    const int64_t rows = (int64_t)depth * kTileN + 1 + s.nq - s.nk;   /* a tile ending at this many rows or more is one */
+    const int rows = depth * kTileN - s.nk + s.nq + 1;   /* a tile ending at this many rows or more is one; depth <= nk / 128 + 1 */
     if (rows > s.nq) return 0;
-    return rows <= 0 ? all : all - (int)((rows + tokens - 1) / tokens - 1);
+    return rows <= 0 ? all : all - ((int)((uint32_t)(rows + tokens - 1) / (uint32_t)tokens) - 1);
 }
 __device__ __forceinline__ int warp_sum(int x) {
 #pragma unroll
@@ -138,57 +138,75 @@ __device__ __forceinline__ int lane_holding(int x, int at, int lane, int* before
     return k;
 }
 
-/* Announces this pair's query tiles in the ring of either CTA; the whole warp 14 of both, which reach the same order by
- * themselves. Up to 32 sequences (a lane each, `mine`) the tiles go from the most key tiles to the fewest over all
- * sequences, in turns back and forth; with more, in the batch's order. */
-__device__ void order_tiles(const Plan& p, Shared& s, const Seq& mine, int rank, int lane) {
-    const RidgeFillAttnPrefill& g = p.g;
-    const int n_seq = (int)g.n_seq, heads = (int)g.n_head_kv, pairs = (int)rf::cluster_count_x(), pair = (int)rf::cluster_id_x();
-    const int tokens = 2 * p.tokens;   /* of a query tile */
-    const bool sorted = n_seq <= 32;
-    int most = mine.nq > 0 ? mine.nk / kTileN + 1 : 0;
+/* The order of this pair's query tiles, the whole warp 14 of both CTAs, which reach the same order by themselves. Up to 32
+ * sequences (a lane each) the tiles go from the most key tiles to the fewest over all sequences, in turns back and forth;
+ * with more, in the batch's order. */
+struct Order {
+    const Plan& p;
+    int rank, lane, heads, pairs, pair, tokens;
+    bool sorted;
+    Seq mine = {};               /* sorted: this lane's sequence */
+    int most = 0, total = 0;     /* the most key tiles of any query tile at most; the query tiles of one kv head */
+    int block = 0, base = 0;     /* unsorted: the block of 32 sequences reached, and the tiles before it */
+    Item own = {};               /* this lane's tile, if it is the owner of the one asked for */
+
+    __device__ __forceinline__ Order(const Plan& plan, int rank_, int lane_) : p(plan), rank(rank_), lane(lane_) {
+        const int n_seq = (int)p.g.n_seq;
+        heads = (int)p.g.n_head_kv;
+        pairs = (int)rf::cluster_count_x();
+        pair = (int)rf::cluster_id_x();
+        tokens = 2 * p.tokens;   /* of a query tile */
+        sorted = n_seq <= 32;
+        if (!sorted) return;
+        if (lane < n_seq) mine = sequence(p.g, lane);
+        most = mine.nq > 0 ? mine.nk / kTileN + 1 : 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const int total = warp_sum(deeper(mine, -1, tokens));
-    int block = 0, base = 0;   /* unsorted: the block of 32 sequences reached, and the tiles before it */
-    for (int k = 0;; ++k) {
+        for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        total = warp_sum(deeper(mine, -1, tokens));
+    }
+
+    /* The lane whose `own` is the pair's k-th query tile; -1: there is none. */
+    __device__ __forceinline__ int find(int k) {
         const int at = sorted && (k & 1) ? k * pairs + pairs - 1 - pair : k * pairs + pair;
-        const int t = at / heads, head = at - t * heads;
-        Item own = {};
-        int owner = -1;
+        const int t = (int)((uint32_t)at / (uint32_t)heads), head = at - t * heads;
+        int before = 0, sum;
         if (sorted) {
-            if (t < total) {
-                int lo = 0, hi = most;   /* the least depth with at most t deeper tiles: tile t has that depth */
-                while (lo < hi) {
-                    const int mid = (lo + hi) >> 1;
-                    if (warp_sum(deeper(mine, mid, tokens)) <= t) hi = mid;
-                    else lo = mid + 1;
-                }
-                const int more = deeper(mine, lo, tokens), same = deeper(mine, lo - 1, tokens) - more;
-                const int in = t - warp_sum(more);
-                int before = 0, sum;
-                owner = max(lane_holding(same, in, lane, &before, &sum), 0);
-                own = tile_of(mine, deeper(mine, -1, tokens) - (more + same) + (in - before), p.tokens, head, rank);
+            if (t >= total) return -1;
+            int lo = 0, hi = most;   /* the least depth with at most t deeper tiles: tile t has that depth */
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (warp_sum(deeper(mine, mid, tokens)) <= t) hi = mid;
+                else lo = mid + 1;
             }
-        } else {
-            for (; block < n_seq; block += 32) {
-                Seq q = {};
-                if (block + lane < n_seq) q = sequence(g, block + lane);
-                int before = 0, sum;
-                owner = lane_holding(deeper(q, -1, tokens), t - base, lane, &before, &sum);
-                if (owner >= 0) {
-                    own = tile_of(q, t - base - before, p.tokens, head, rank);
-                    break;
-                }
-                base += sum;
-            }
+            const int more = deeper(mine, lo, tokens), same = deeper(mine, lo - 1, tokens) - more;
+            const int in = t - warp_sum(more);
+            const int owner = max(lane_holding(same, in, lane, &before, &sum), 0);
+            own = tile_of(mine, deeper(mine, -1, tokens) - (more + same) + (in - before), p.tokens, head, rank);
+            return owner;
         }
+        for (; block < (int)p.g.n_seq; block += 32) {
+            Seq q = {};
+            if (block + lane < p.g.n_seq) q = sequence(p.g, block + lane);
+            const int owner = lane_holding(deeper(q, -1, tokens), t - base, lane, &before, &sum);
+            if (owner >= 0) {
+                own = tile_of(q, t - base - before, p.tokens, head, rank);
+                return owner;
+            }
+            base += sum;
+        }
+        return -1;
+    }
+};
+
+/* Announces them in the ring; `owner`: the first one's, found before the barriers stood. */
+__device__ void announce(Order& order, Shared& s, int owner) {
+    for (int k = 0;; owner = order.find(++k)) {
         const int slot = k % kRing;
         if (!rf::mbar_wait(&s.item_empty[slot], ((k / kRing) & 1) ^ 1, &s.abort, rf::kErrAttnWait)) return;
         __syncwarp();
-        if (owner < 0) own.rows = -1;
-        if (lane == max(owner, 0)) {
-            s.item[slot] = own;
+        if (owner < 0) order.own.rows = -1;
+        if (order.lane == max(owner, 0)) {
+            s.item[slot] = order.own;
             rf::mbar_arrive(&s.item_full[slot]);
         }
         if (owner < 0) return;
@@ -325,7 +343,7 @@ __device__ void multiply(Shared& s, const uint8_t* qtile, const uint8_t* ring, u
             const bool last = j + 1 == it.tiles, cut = last && it.tiles * kTileN > it.keys;
             if (cut) {   /* the last V rows have landed: those past the sequence may be cleared, in both CTAs */
                 if (!wait(full(v), phase(v), full(v + 1), phase(v + 1), full(v), phase(v), full(v), phase(v))) break;
-                if (lane < 2) rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.v_last), lane));
+                if (lane < 2) rf::mbar_arrive_remote(rf::map_rank(rf::smem_addr(&s.v_last), lane));
                 __syncwarp();
             }
             uint64_t* p = &s.p_full[tile & 1];
@@ -485,7 +503,7 @@ __device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, u
             }
             rf::fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.v_clean), 0));
+            if (lane == 0) rf::mbar_arrive_remote(rf::map_rank(rf::smem_addr(&s.v_clean), 0));
         }
         bool ok = rf::mbar_wait(&s.o_full, done & 1, &s.abort, rf::kErrAttnWait);
         if (ok) ok = rf::mbar_wait(&s.sum_full[done % 3], (done / 3) & 1, &s.abort, rf::kErrAttnWait);
@@ -537,8 +555,6 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     uint8_t* turn = ring + kStages * kStageBytes;
     Shared& s = *(Shared*)(turn + kOutWarps * kTurnBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)rf::cluster_rank();
-    Seq mine = {};   /* the ordering warp's first loads, before the barriers stand */
-    if (warp == kWarps - 1 && p.g.n_seq <= 32 && lane < p.g.n_seq) mine = sequence(p.g, lane);
     if (threadIdx.x == 0) {
         for (int i = 0; i < kRing; ++i) {
             rf::mbar_init(&s.item_full[i], 1);
@@ -569,6 +585,14 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         rf::tma_prefetch_map(&map_v);
     }
     if (warp == 13) rf::tmem_alloc_pair<kTmemCols>(&s.tmem);
+    if (warp == 14) {   /* the first query tile is found while the barriers are made */
+        Order order(p, rank, lane);
+        const int owner = order.find(0);
+        rf::cluster_sync_all();
+        announce(order, s, owner);
+        rf::cluster_sync_all();
+        return;
+    }
     rf::tc_fence_before();
     rf::cluster_sync_all();   /* both CTAs' barriers are initialised before either signals the other's */
     rf::tc_fence_after();
@@ -576,7 +600,6 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     if (warp < 8) soften(p, s, tmem, warp, lane);
     else if (warp < 12) output(p, s, ring, turn, tmem, warp - 8, lane);
     else if (warp == 12) produce(p, s, qtile, ring, &map_q, &map_k, &map_v, rank, lane);
-    else if (warp == 14) order_tiles(p, s, mine, rank, lane);
     else if (rank == 0) multiply(s, qtile, ring, tmem, lane);
     rf::tc_fence_before();
     rf::cluster_sync_all();   /* no product reads the other CTA's memory any more */

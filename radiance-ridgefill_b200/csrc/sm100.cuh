@@ -313,6 +313,12 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t caddr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(caddr) : "memory");
 }
 
+/* The same arrival ordering only what this thread wrote within its own CTA (release at CTA scope, without the fence over the
+ * cluster that costs about a microsecond): for hand-overs whose data the reader takes from the arriving CTA's memory. */
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t caddr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(caddr) : "memory");
+}
+
 /* Packed f32x2 arithmetic (sm_100): two lanes of f32 per instruction, each rounded as its scalar form. */
 __device__ __forceinline__ void fma2_rn(float& a0, float& a1, float x0, float x1, float y0, float y1) {   /* a = x * y + a */
     asm("{\n .reg .b64 a, x, y;\n mov.b64 a, {%0, %1};\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"

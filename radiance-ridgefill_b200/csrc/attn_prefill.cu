@@ -21,7 +21,7 @@
  *               exponentials, sums, P. The running maximum is followed only when a tile exceeds it by 2^8: rescaling O,
  *               256 columns of tensor memory a row, is then rare, and the weights of a row stay below 2^8
  *   warps 8-11  the output: O from tensor memory, divided by the row's sum, rounded once to bf16, turned in shared memory
- *               so that four lanes write 64 bytes of a row, while the next query tile's products run; and, where a
+ *               so that eight lanes write 128 bytes of a row, while the next query tile's products run; and, where a
  *               sequence's last key tile is not full, the zeroing of its V rows past the end (another sequence's rows, or
  *               anything behind the last one: P is zero there, but a NaN times zero is not)
  *   warp 12     TMA loads     warp 13  the products' issue (the pair's first CTA)     warp 14  the order of the tiles
@@ -36,10 +36,10 @@
 namespace {
 
 constexpr int D = 256, kTileM = 128, kTileN = 128;           /* rows of a CTA (the pair's tile has 256); keys */
-constexpr int kStages = 9, kStageBytes = 16384, kQBytes = kTileM * D * 2;
+constexpr int kStages = 8, kStageBytes = 16384, kQBytes = kTileM * D * 2;
 constexpr int kBoxBytes = 64 * 64 * 2;                       /* one TMA box of K or V: 64 rows x 64 elements */
 constexpr int kSoftWarps = 8, kOutWarps = 4, kWarps = kSoftWarps + kOutWarps + 3, kThreads = 32 * kWarps;
-constexpr int kTurnBytes = 32 * 64;                          /* an output warp's 32 rows x 32 elements */
+constexpr int kTurnBytes = 32 * 128;                         /* an output warp's 32 rows x 64 elements */
 constexpr int kRing = 4;                                     /* query tiles announced ahead */
 constexpr uint32_t kTmemCols = 512, kColO = 256;
 constexpr float kGrow = 8.0f, kNone = -INFINITY;
@@ -61,6 +61,7 @@ struct Item {
 
 struct Shared {
     Item item[kRing];
+    int64_t at[kTileM];                    /* where row r of the CTA's lies in o, from the first one's place */
     float top[2][2][kTileM];               /* rows' maxima of a tile's two halves, by the tile's parity */
     float sum[3][2][kTileM];               /* rows' sums (two halves) of the query tiles under way */
     uint64_t item_full[kRing], item_empty[kRing];
@@ -482,12 +483,9 @@ __device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, u
         const Item it = items.next(lane);
         if (it.rows < 0) return;
         const int live = it.rows * p.group;   /* this CTA's rows */
-        auto row_at = [&](int r) {
-            const int token = r / p.group;
-            return g.o + (int64_t)(it.q0 + token) * g.o_row + (int64_t)(it.head * p.group + r - token * p.group) * g.o_head;
-        };
+        uint16_t* const out = g.o + (int64_t)it.q0 * g.o_row + (int64_t)(it.head * p.group) * g.o_head;
         if (it.tiles == 0) {   /* no row of the tile has a key */
-            for (int r = warp * 32; r < min(warp * 32 + 32, live); ++r) *(uint4*)(row_at(r) + 8 * lane) = make_uint4(0u, 0u, 0u, 0u);
+            for (int r = warp * 32; r < min(warp * 32 + 32, live); ++r) *(uint4*)(out + s.at[r] + 8 * lane) = make_uint4(0u, 0u, 0u, 0u);
             continue;
         }
         use += 4 * it.tiles;
@@ -512,34 +510,42 @@ __device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, u
         const float sum = s.sum[done % 3][0][row] + s.sum[done % 3][1][row];
         const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);   /* no key: zeros; a NaN stays one */
         uint8_t* tile = turn + warp * kTurnBytes;
-        uint16_t* dst[4];   /* this lane's chunk of the four rows it writes */
+        uint16_t* dst[8];   /* this lane's chunk of the eight rows it writes */
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dst[i] = row_at(warp * 32 + 8 * i + (lane >> 2)) + 8 * (lane & 3);
-#pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {   /* 32 elements of the 32 rows: 16-byte chunk v of row r at chunk v ^ (r / 2 % 4) */
-            uint32_t o[32];
-            rf::tmem_ld32(mine + 32 * c, o);
+        for (int i = 0; i < 8; ++i) dst[i] = out + s.at[warp * 32 + 4 * i + (lane >> 3)] + 8 * (lane & 7);
+        const int rows = live - warp * 32 - (lane >> 3);   /* row i of them is one of the tile's while 4 i < rows */
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {   /* 64 elements of the 32 rows: 16-byte chunk v of row r at chunk v ^ (r & 7) */
+            uint32_t o[2][32];
+            rf::tmem_ld32(mine + 64 * c, o[0]);
+            rf::tmem_ld32(mine + 64 * c + 32, o[1]);
             rf::tmem_ld_wait();
-            if (c + 1 == D / 32) {   /* O's last read */
+            if (c + 1 == D / 64) {   /* O's last read */
                 rf::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) rf::mbar_arrive_cluster_relaxed(rf::map_rank(rf::smem_addr(&s.o_empty), 0));
             }
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
+            for (int v = 0; v < 8; ++v) {
                 uint32_t w[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    w[e] = pack(__uint_as_float(o[8 * v + 2 * e]) * inv, __uint_as_float(o[8 * v + 2 * e + 1]) * inv);
-                *(uint4*)(tile + lane * 64 + ((v ^ (lane >> 1 & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int e = 0; e < 4; ++e) {
+                    const int x = 8 * (v & 3) + 2 * e;
+                    w[e] = pack(__uint_as_float(o[v >> 2][x]) * inv, __uint_as_float(o[v >> 2][x + 1]) * inv);
+                }
+                *(uint4*)(tile + lane * 128 + ((v ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
             __syncwarp();
+            uint4 t[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = 8 * i + (lane >> 2), v = lane & 3;
-                if (warp * 32 + r < live) *(uint4*)(dst[i] + 32 * c) = *(const uint4*)(tile + r * 64 + ((v ^ (r >> 1 & 3)) << 4));
+            for (int i = 0; i < 8; ++i) {
+                const int r = 4 * i + (lane >> 3);
+                t[i] = *(const uint4*)(tile + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
             }
-            __syncwarp();   /* read before the next 32 elements take its place */
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (4 * i < rows) *(uint4*)(dst[i] + 64 * c) = t[i];
+            __syncwarp();   /* read before the next 64 elements take its place */
         }
         ++done;
     }
@@ -583,6 +589,10 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         rf::tma_prefetch_map(&map_q);
         rf::tma_prefetch_map(&map_k);
         rf::tma_prefetch_map(&map_v);
+    }
+    if (threadIdx.x >= 128 && threadIdx.x < 128 + kTileM) {
+        const int r = threadIdx.x - 128, token = r / p.group;
+        s.at[r] = (int64_t)token * p.g.o_row + (int64_t)(r - token * p.group) * p.g.o_head;
     }
     if (warp == 13) rf::tmem_alloc_pair<kTmemCols>(&s.tmem);
     if (warp == 14) {   /* the first query tile is found while the barriers are made */

@@ -101,6 +101,7 @@ int ridgefill_attn_decode_device(const RadArgs* a, RadStream s);
 int ridgefill_gdn_step_device(const RadArgs* a, RadStream s);
 
 /* Scratch hooks: device bytes the call needs in RadArgs::scratch (16-byte aligned); 0: none. */
+int64_t ridgefill_attn_prefill_scratch(const RadArgs* a);
 int64_t ridgefill_attn_decode_scratch(const RadArgs* a);
 
 #ifdef __cplusplus

@@ -10,7 +10,7 @@
  * A CTA's 128 rows are the 128 / group tokens' rows of all `group` query heads of one kv head, the pair's second CTA
  * taking the next tokens: a key tile is read once for the whole group, and the causal edge cuts at 2 x 128 / group rows,
  * not at 256. Persistent pairs take query tiles from the longest to the shortest, in turns that run back and forth, so
- * that their sums are near alike.
+ * that their sums are near alike; few query tiles over long keys are split along the keys instead (Spans).
  *
  * Tensor memory (512 columns a CTA): two 128-column buffers of scores, and O's 256. P, rounded to bf16, replaces its
  * scores in place (64 columns) and is the second product's A operand from there. Shared memory: Q's 64 KiB and a ring of
@@ -51,18 +51,28 @@ struct Plan {
     RidgeFillAttnPrefill g;
     int group, tokens;      /* query heads a kv head; tokens of a CTA's rows (128 / group) */
     float scale_log2;
+    void* partials;         /* split over the keys: [pairs][2 slots][2 CTAs] Partial; null: whole query tiles */
+    int pairs;              /* of the split */
 };
 
-/* One query tile as a CTA sees it: `rows` tokens of its own from row q0 of q, keys from row k0 of k and v, `tiles` key
- * tiles (the pair's); its token t sees the sequence's keys 0 .. limit + t, of which there are `keys`. rows < 0: no more. */
+/* A CTA's part of a query tile's result: O's sums by column, and the rows' maxima (log2 units) and sums of weights. */
+struct Partial {
+    float o[D][kTileM];
+    float2 ml[kTileM];
+};
+
+/* One query tile as a CTA sees it: `rows` tokens of its own from row q0 of q, keys from row k0 of k and v, key tiles first
+ * .. first + tiles - 1 (the pair's); its token t sees the sequence's keys 0 .. limit + t, of which there are `keys`. slot
+ * -1: all of its key tiles, the output is written; 0, 1: a piece, its Partial goes to that slot. rows < 0: no more. */
 struct Item {
-    int q0, rows, k0, keys, tiles, limit, head;
+    int q0, rows, k0, keys, first, tiles, limit, head, slot;
 };
 
 struct Shared {
     Item item[kRing];
     int64_t at[kTileM];                    /* where row r of the CTA's lies in o, from the first one's place */
     float top[2][2][kTileM];               /* rows' maxima of a tile's two halves, by the tile's parity */
+    float top_of[3][kTileM];               /* and the maxima they go by */
     float sum[3][2][kTileM];               /* rows' sums (two halves) of the query tiles under way */
     uint64_t item_full[kRing], item_empty[kRing];
     uint64_t q_full, q_empty, kv_full[kStages], kv_empty[kStages];
@@ -106,8 +116,10 @@ __device__ __forceinline__ Item tile_of(const Seq& s, int i, int tokens, int hea
     t.keys = s.nk;
     t.limit = s.nk - s.nq + from + rank * tokens;
     const int last = s.nk - s.nq + from + both - 1;   /* the pair's last row's last key */
+    t.first = 0;
     t.tiles = last < 0 ? 0 : last / kTileN + 1;
     t.head = head;
+    t.slot = -1;
     return t;
 }
 /* How many query tiles of a sequence have more than `depth` key tiles: the last ones. depth -1: all. */
@@ -139,9 +151,43 @@ __device__ __forceinline__ int lane_holding(int x, int at, int lane, int* before
     return k;
 }
 
+/* ------------------------------------------------------------------ the split over the keys
+ * All key tiles of all query tiles in a row -- sequence, query tile, kv head, key -- cut into equal spans, one a pair. A
+ * span that holds all key tiles of a query tile writes its output; the at most two that it cuts leave Partials (slot 1 of
+ * the pair that has the first of them, slot 0 of the others), which join_kernel adds up. */
+struct Spans {
+    int n, each, extra;   /* the first `extra` spans one longer; with few tiles fewer spans, of four at least */
+    __device__ __forceinline__ Spans(int total, int most) {
+        n = max(min((total + 3) / 4, most), 1);
+        each = total / n;
+        extra = total - each * n;
+    }
+    __device__ __forceinline__ int first(int i) const { return i * each + min(i, extra); }
+    __device__ __forceinline__ int owner(int u) const {
+        const int longer = extra * (each + 1);
+        return u < longer ? u / (each + 1) : extra + (u - longer) / each;
+    }
+};
+
+/* Query tile `i` of a sequence has this many key tiles (0 past its last one). */
+__device__ __forceinline__ int depth_of(const Seq& q, int i, int tokens) {
+    return i * 2 * tokens < q.nq ? tile_of(q, i, tokens, 0, 0).tiles : 0;
+}
+
+/* Walks the query tiles in order, 32 at a time; `at`(sequence, first query tile, this lane's key tiles of one head) is asked
+ * for each 32 and ends the walk by answering true. The whole warp. */
+template <class F>
+__device__ __forceinline__ void walk(const Plan& p, int lane, F&& at) {
+    for (int q = 0; q < (int)p.g.n_seq; ++q) {
+        const Seq s = sequence(p.g, q);
+        for (int i = 0; i * 2 * p.tokens < s.nq; i += 32)
+            if (at(s, i, depth_of(s, i + lane, p.tokens))) return;
+    }
+}
+
 /* The order of this pair's query tiles, the whole warp 14 of both CTAs, which reach the same order by themselves. Up to 32
  * sequences (a lane each) the tiles go from the most key tiles to the fewest over all sequences, in turns back and forth;
- * with more, in the batch's order. */
+ * with more, in the batch's order. Split over the keys: the pieces of the pair's span. */
 struct Order {
     const Plan& p;
     int rank, lane, heads, pairs, pair, tokens;
@@ -149,6 +195,7 @@ struct Order {
     Seq mine = {};               /* sorted: this lane's sequence */
     int most = 0, total = 0;     /* the most key tiles of any query tile at most; the query tiles of one kv head */
     int block = 0, base = 0;     /* unsorted: the block of 32 sequences reached, and the tiles before it */
+    int unit = 0, end = 0;       /* split: the rest of the span */
     Item own = {};               /* this lane's tile, if it is the owner of the one asked for */
 
     __device__ __forceinline__ Order(const Plan& plan, int rank_, int lane_) : p(plan), rank(rank_), lane(lane_) {
@@ -157,7 +204,21 @@ struct Order {
         pairs = (int)rf::cluster_count_x();
         pair = (int)rf::cluster_id_x();
         tokens = 2 * p.tokens;   /* of a query tile */
-        sorted = n_seq <= 32;
+        sorted = n_seq <= 32 && !p.partials;
+        if (p.partials) {
+            int units = 0;
+            walk(p, lane, [&](const Seq&, int, int depth) {
+                units += depth;
+                return false;
+            });
+            units = warp_sum(units) * heads;
+            const Spans spans(units, p.pairs);
+            if (pair < spans.n) {
+                unit = spans.first(pair);
+                end = spans.first(pair + 1);
+            }
+            return;
+        }
         if (!sorted) return;
         if (lane < n_seq) mine = sequence(p.g, lane);
         most = mine.nq > 0 ? mine.nk / kTileN + 1 : 0;
@@ -166,8 +227,32 @@ struct Order {
         total = warp_sum(deeper(mine, -1, tokens));
     }
 
+    /* The lane whose `own` is the next piece of the span; -1: there is none. */
+    __device__ __forceinline__ int piece() {
+        if (unit >= end) return -1;
+        int owner = -1, done = 0, used = 0;
+        walk(p, lane, [&](const Seq& s, int i, int depth) {
+            int before = 0, sum = 0;
+            owner = lane_holding(depth * heads, unit - done, lane, &before, &sum);
+            if (owner < 0) {
+                done += sum;
+                return false;
+            }
+            const int tiles = __shfl_sync(0xffffffffu, depth, owner), in = unit - done - before, head = in / tiles;
+            own = tile_of(s, i + owner, p.tokens, head, rank);
+            own.first = in - head * tiles;
+            own.tiles = min(tiles - own.first, end - unit);
+            own.slot = own.tiles == tiles ? -1 : own.first > 0 ? 0 : 1;
+            used = own.tiles;
+            return true;
+        });
+        unit = owner < 0 ? end : unit + used;
+        return owner;
+    }
+
     /* The lane whose `own` is the pair's k-th query tile; -1: there is none. */
     __device__ __forceinline__ int find(int k) {
+        if (p.partials) return piece();
         const int at = sorted && (k & 1) ? k * pairs + pairs - 1 - pair : k * pairs + pair;
         const int t = (int)((uint32_t)at / (uint32_t)heads), head = at - t * heads;
         int before = 0, sum;
@@ -266,9 +351,9 @@ __device__ void produce(const Plan& p, Shared& s, uint8_t* qtile, uint8_t* ring,
             }
             for (int j = 0; j <= it.tiles; ++j) {
                 if (j < it.tiles)   /* this CTA's 64 keys of the tile */
-                    for (int h = 0; h < 2; ++h) stage(map_k, h * 128, it.k0 + j * kTileN + rank * 64);
+                    for (int h = 0; h < 2; ++h) stage(map_k, h * 128, it.k0 + (it.first + j) * kTileN + rank * 64);
                 if (j > 0)          /* the tile's keys, this CTA's 128 elements */
-                    for (int h = 0; h < 2; ++h) stage(map_v, rank * 128, it.k0 + (j - 1) * kTileN + h * 64);
+                    for (int h = 0; h < 2; ++h) stage(map_v, rank * 128, it.k0 + (it.first + j - 1) * kTileN + h * 64);
             }
         }
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
@@ -317,6 +402,7 @@ __device__ void multiply(Shared& s, const uint8_t* qtile, const uint8_t* ring, u
                 ahead.rows = __shfl_sync(0xffffffffu, i.rows, 0);
                 ahead.tiles = __shfl_sync(0xffffffffu, i.tiles, 0);
                 ahead.keys = __shfl_sync(0xffffffffu, i.keys, 0);
+                ahead.first = __shfl_sync(0xffffffffu, i.first, 0);
             } while (ahead.rows >= 0 && ahead.tiles == 0);
             ja = 0;
         }
@@ -341,7 +427,7 @@ __device__ void multiply(Shared& s, const uint8_t* qtile, const uint8_t* ring, u
             use += 2;
         }
         if (j >= 0) {
-            const bool last = j + 1 == it.tiles, cut = last && it.tiles * kTileN > it.keys;
+            const bool last = j + 1 == it.tiles, cut = last && (it.first + it.tiles) * kTileN > it.keys;
             if (cut) {   /* the last V rows have landed: those past the sequence may be cleared, in both CTAs */
                 if (!wait(full(v), phase(v), full(v + 1), phase(v + 1), full(v), phase(v), full(v), phase(v))) break;
                 if (lane < 2) rf::mbar_arrive_remote(rf::map_rank(rf::smem_addr(&s.v_last), lane));
@@ -403,8 +489,9 @@ __device__ void soften(const Plan& p, Shared& s, uint32_t tmem, int warp, int la
 #pragma unroll
             for (int c = 0; c < 2; ++c) rf::tmem_ld32(at + 64 * half + 32 * c, x[c]);
             rf::tmem_ld_wait();
-            if (j * kTileN + 64 * half + 63 > it.limit) {   /* the first token does not see all of these keys */
-                const int last = limit - j * kTileN - 64 * half;
+            const int key = (it.first + j) * kTileN + 64 * half;
+            if (key + 63 > it.limit) {   /* the first token does not see all of these keys */
+                const int last = limit - key;
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -460,7 +547,10 @@ __device__ void soften(const Plan& p, Shared& s, uint32_t tmem, int warp, int la
             /* The row's sum, announced before the last P so that no warp can be a query tile ahead of another here. Three
              * buffers: these scores may come before the last PV of the query tile before, but not before that of the one
              * before it, whose first PV waited for O's reader to be done with the buffer's earlier sums. */
-            if (j + 1 == it.tiles) s.sum[buf][half][row] = l0 + l1;
+            if (j + 1 == it.tiles) {
+                s.sum[buf][half][row] = l0 + l1;
+                if (half == 0) s.top_of[buf][row] = m;
+            }
             rf::tmem_st_wait();
             rf::tc_fence_before();
             __syncwarp();
@@ -473,7 +563,7 @@ __device__ void soften(const Plan& p, Shared& s, uint32_t tmem, int warp, int la
     }
 }
 
-__device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, uint32_t tmem, int warp, int lane) {
+__device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, uint32_t tmem, int rank, int warp, int lane) {
     const RidgeFillAttnPrefill& g = p.g;
     Items items{ s };
     uint32_t use = 0, done = 0, partial = 0;
@@ -489,10 +579,10 @@ __device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, u
             continue;
         }
         use += 4 * it.tiles;
-        if (it.tiles * kTileN > it.keys) {   /* V rows of the last tile past the sequence: the last two stages, 64 rows each */
+        if ((it.first + it.tiles) * kTileN > it.keys) {   /* V rows of the last tile past the sequence: the last two stages, 64 rows each */
             const bool ok = rf::mbar_wait(&s.v_last, partial++ & 1, &s.abort, rf::kErrAttnWait);
             if (!__all_sync(0xffffffffu, ok)) return;
-            if ((it.tiles - 1) * kTileN + row >= it.keys) {
+            if ((it.first + it.tiles - 1) * kTileN + row >= it.keys) {
                 uint8_t* at = ring + ((use - 2 + (uint32_t)(row >> 6)) % kStages) * kStageBytes + (row & 63) * 128;
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
@@ -508,6 +598,23 @@ __device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, u
         if (!__all_sync(0xffffffffu, ok)) return;
         rf::tc_fence_after();
         const float sum = s.sum[done % 3][0][row] + s.sum[done % 3][1][row];
+        if (it.slot >= 0) {   /* a piece: a thread its row's sums, a column's 128 rows side by side */
+            Partial& part = ((Partial*)p.partials)[((int64_t)rf::cluster_id_x() * 2 + it.slot) * 2 + rank];
+            part.ml[row] = make_float2(s.top_of[done % 3][row], sum);
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                rf::tmem_ld32(mine + 32 * c, o);
+                rf::tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) part.o[32 * c + e][row] = __uint_as_float(o[e]);
+            }
+            rf::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) rf::mbar_arrive_cluster_relaxed(rf::map_rank(rf::smem_addr(&s.o_empty), 0));
+            ++done;
+            continue;
+        }
         const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);   /* no key: zeros; a NaN stays one */
         uint8_t* tile = turn + warp * kTurnBytes;
         uint16_t* dst[8];   /* this lane's chunk of the eight rows it writes */
@@ -590,6 +697,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         rf::tma_prefetch_map(&map_k);
         rf::tma_prefetch_map(&map_v);
     }
+    if (p.partials) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   /* the join may line up */
     if (threadIdx.x >= 128 && threadIdx.x < 128 + kTileM) {
         const int r = threadIdx.x - 128, token = r / p.group;
         s.at[r] = (int64_t)token * p.g.o_row + (int64_t)(r - token * p.group) * p.g.o_head;
@@ -608,13 +716,91 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     rf::tc_fence_after();
     const uint32_t tmem = s.tmem;
     if (warp < 8) soften(p, s, tmem, warp, lane);
-    else if (warp < 12) output(p, s, ring, turn, tmem, warp - 8, lane);
+    else if (warp < 12) output(p, s, ring, turn, tmem, rank, warp - 8, lane);
     else if (warp == 12) produce(p, s, qtile, ring, &map_q, &map_k, &map_v, rank, lane);
     else if (rank == 0) multiply(s, qtile, ring, tmem, lane);
     rf::tc_fence_before();
     rf::cluster_sync_all();   /* no product reads the other CTA's memory any more */
     rf::tc_fence_after();
     if (warp == 13) rf::tmem_free_pair<kTmemCols>(tmem);
+}
+
+constexpr int kJoinCols = 64, kJoinParts = D / kJoinCols;
+
+/* The query tiles that the split cut, and those without a key (zeros): a CTA joins kJoinCols columns of a CTA's share of
+ * one query tile and kv head, a thread a row. */
+__global__ void __launch_bounds__(kTileM) join_kernel(const Plan p) {
+    const RidgeFillAttnPrefill& g = p.g;
+    const int lane = threadIdx.x & 31, row = threadIdx.x, heads = (int)g.n_head_kv;
+    const int part = blockIdx.x % kJoinParts, rank = blockIdx.x / kJoinParts % 2, item = blockIdx.x / (2 * kJoinParts);
+    const int query = item / heads, head = item - query * heads;
+    int seen = 0, units = 0, start = 0, tiles = -1;
+    Item it = {};
+    walk(p, lane, [&](const Seq& s, int i, int depth) {
+        const int here = min(32, (s.nq + 2 * p.tokens - 1) / (2 * p.tokens) - i), in = query - seen;
+        if (in >= 0 && in < here) {   /* the query tile is one of these 32 */
+            it = tile_of(s, i + in, p.tokens, head, rank);
+            tiles = it.tiles;
+            start = (units + warp_sum(lane < in ? depth : 0)) * heads + head * tiles;
+        }
+        seen += here;
+        units += warp_sum(depth);
+        return false;
+    });
+    if (tiles < 0) return;   /* fewer query tiles than the grid has places for */
+    const int token = row / p.group;
+    uint16_t* out = g.o + (int64_t)(it.q0 + token) * g.o_row + (int64_t)(head * p.group + row - token * p.group) * g.o_head + part * kJoinCols;
+    const bool live = token < it.rows;
+    if (tiles == 0) {
+        if (live)
+            for (int c = 0; c < kJoinCols / 8; ++c) *(uint4*)(out + 8 * c) = make_uint4(0u, 0u, 0u, 0u);
+        return;
+    }
+    const Spans spans(units * heads, p.pairs);
+    const int c0 = spans.owner(start), n = spans.owner(start + tiles - 1) - c0 + 1;
+    if (n == 1) return;   /* written by its one pair */
+    asm volatile("griddepcontrol.wait;" ::: "memory");   /* the split is done and its results are visible */
+    auto piece = [&](int i) -> const Partial& { return ((const Partial*)p.partials)[((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * 2 + rank]; };
+    float top = kNone, sum = 0.f, acc[kJoinCols];
+    for (int i = 0; i < n; ++i) top = fmaxf(top, piece(i).ml[row].x);
+#pragma unroll
+    for (int c = 0; c < kJoinCols; ++c) acc[c] = 0.f;
+    for (int i = 0; i < n; ++i) {
+        const Partial& s = piece(i);
+        const float2 ml = s.ml[row];
+        const float f = ml.x == kNone ? 0.f : exp2_approx(ml.x - top);
+        sum = fmaf(f, ml.y, sum);
+#pragma unroll
+        for (int c = 0; c < kJoinCols; ++c) acc[c] = fmaf(f, s.o[part * kJoinCols + c][row], acc[c]);
+    }
+    if (!live) return;
+    const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
+#pragma unroll
+    for (int c = 0; c < kJoinCols; c += 8)
+        *(uint4*)(out + c) = make_uint4(pack(acc[c] * inv, acc[c + 1] * inv), pack(acc[c + 2] * inv, acc[c + 3] * inv),
+                                        pack(acc[c + 4] * inv, acc[c + 5] * inv), pack(acc[c + 6] * inv, acc[c + 7] * inv));
+}
+
+/* How a parsed call runs. Query tiles go to pairs whole where there are many; with two a pair or fewer and long keys (the
+ * tail of a long prompt) that would leave pairs idle -- 128 query tiles of 256 key tiles on 74 pairs take two rounds, 86 % of
+ * the pairs' time -- so the key tiles are split evenly instead, and the cut query tiles joined. */
+constexpr int kLongKeys = 8192;
+struct Shape {
+    int group, tokens;
+    int64_t items;      /* query tiles (of all kv heads) at most: a sequence's last one may be cut short */
+    int pairs;
+    bool split;
+    int64_t bytes;
+};
+Shape shape_of(const RidgeFillAttnPrefill& g) {
+    Shape s;
+    s.group = (int)(g.n_head / g.n_head_kv);
+    s.tokens = kTileM / s.group;
+    s.items = (g.T / (2 * s.tokens) + g.n_seq) * g.n_head_kv;
+    s.pairs = rf::sm_count() / 2;
+    s.split = g.Tk >= kLongKeys && s.items <= 2 * s.pairs;
+    s.bytes = s.split ? (int64_t)s.pairs * 4 * (int64_t)sizeof(Partial) : 0;
+    return s;
 }
 
 /* Head rows [T, heads, 256] bf16 as a 3-D tensor map read in boxes of 64 elements x `heads_box` heads x `rows_box` rows,
@@ -640,18 +826,25 @@ namespace rf {
 int attn_device_error(int reset) { return read_device_error(reset); }
 }  // namespace rf
 
+extern "C" int64_t ridgefill_attn_prefill_scratch(const RadArgs* a) {
+    RidgeFillAttnPrefill g;
+    return ridgefill_attn_prefill_parse(a, &g) == RAD_OK && g.T > 0 && g.n_seq > 0 ? shape_of(g).bytes : 0;
+}
+
 extern "C" int ridgefill_attn_prefill_device(const RadArgs* a, RadStream s) {
     Plan p;
     const int rc = ridgefill_attn_prefill_parse(a, &p.g);
     if (rc != RAD_OK) return rc;
     const RidgeFillAttnPrefill& g = p.g;
     if (g.T == 0 || g.n_seq == 0) return RAD_OK;
-    p.group = (int)(g.n_head / g.n_head_kv);
-    p.tokens = kTileM / p.group;
+    const Shape sh = shape_of(g);
+    if (sh.items > 0x3fffffffLL || (sh.split && sh.items * (g.Tk / kTileN + 1) > 0x7fffffffLL)) return RAD_E_SHAPE;
+    if (sh.split && (!a->scratch || a->scratch_bytes < sh.bytes || (uintptr_t)a->scratch % 16)) return RAD_E_INVAL;
+    p.group = sh.group;
+    p.tokens = sh.tokens;
     p.scale_log2 = g.scale * 1.4426950408889634f;
-    /* query tiles at most: a sequence's last one may be cut short */
-    const int64_t items = (g.T / (2 * p.tokens) + g.n_seq) * g.n_head_kv;
-    if (items > 0x3fffffffLL) return RAD_E_SHAPE;
+    p.partials = sh.split ? a->scratch : nullptr;
+    p.pairs = sh.pairs;
     CUtensorMap mq, mk, mv;
     if (!head_map(&mq, g.q, g.T, g.n_head, g.q_row, g.q_head, p.group, p.tokens)) return RAD_E_DEVICE;
     /* without a key row nothing is read through the maps of k and v */
@@ -662,7 +855,21 @@ extern "C" int ridgefill_attn_prefill_device(const RadArgs* a, RadStream s) {
         cudaGetLastError();
         return RAD_E_DEVICE;
     }
-    const int64_t pairs = rf::sm_count() / 2;
-    prefill_kernel<<<2 * (unsigned)(items < pairs ? items : pairs), kThreads, kSmemBytes, rf::as_stream(s)>>>(mq, mk, mv, p);
-    return rf::launch_status();
+    const int64_t pairs = sh.split || sh.items > sh.pairs ? sh.pairs : sh.items;
+    prefill_kernel<<<2 * (unsigned)pairs, kThreads, kSmemBytes, rf::as_stream(s)>>>(mq, mk, mv, p);
+    if (const int launched = rf::launch_status(); launched != RAD_OK || !sh.split) return launched;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(sh.items * 2 * kJoinParts));
+    cfg.blockDim = dim3(kTileM);
+    cfg.stream = rf::as_stream(s);
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, join_kernel, p) != cudaSuccess) {
+        cudaGetLastError();
+        return RAD_E_DEVICE;
+    }
+    return RAD_OK;
 }

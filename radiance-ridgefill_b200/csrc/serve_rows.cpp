@@ -120,7 +120,7 @@ const RadKernelInfo kServeRows[] = {
               "tcgen05 kind::f16 into tensor memory, TMA-fed: 128 rows (all query heads of a kv head side by side) x 128 keys a "
               "tile, the weights back into tensor memory as the second product's operand, persistent CTAs, longest tiles first",
               "head_dim 256, up to 128 query heads a kv head", "bf16 q / k / v / o, i32 cu_seqlens / cu_keys",
-              ridgefill_attn_prefill_device, nullptr, shape_prefill),
+              ridgefill_attn_prefill_device, ridgefill_attn_prefill_scratch, shape_prefill),
     SERVE_ROW("ridgefill_attn_decode_sm100", "ridgefill_attn_decode",
               "the keys of all sequences split evenly over the SMs, each warp streaming its 16-key blocks through its own "
               "shared-memory ring into mma.sync; the pieces of a sequence joined by a second kernel",

@@ -97,6 +97,29 @@ def test_packed_sequences(cuda, product_lib, nq):
     check(torch, d)
 
 
+@pytest.mark.parametrize("nq,nk", [([1], [9000]), ([40], [8192]), ([300], [20001]), ([2048], [9000]), ([100, 3, 0, 64], [5000, 3, 0, 8200]),
+                                   ([50, 20, 33], [10000, 0, 20]), ([9000 - 8000, 700], [1000, 8300]), ([1] * 40, [700 + 13 * i for i in range(40)])])
+def test_split_over_long_keys(cuda, product_lib, nq, nk):
+    """Few rows over long keys: the key tiles cut into spans, the cut query tiles joined; rows without keys, short and empty
+    sequences beside them."""
+    torch = cuda
+    d = inputs(torch, 80 + sum(nq), nq, nk, 16, 2, pad=3)
+    ops, keep = operands(torch, d)
+    row = product_lib.find_row("ridgefill_attn_prefill", abi.DOMAIN_DEVICE)
+    assert product_lib.scratch_bytes(row, ops, S.prefill_params(d["q"].shape[0], 16, 2)) > 0
+    assert product_lib.launch(row, ops, S.prefill_params(d["q"].shape[0], 16, 2)) == abi.E_INVAL      # without its workspace
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, d, heads=None if sum(nq) < 500 else [0, 5, 8, 15])
+
+
+@pytest.mark.parametrize("hq,hkv", [(3, 1), (12, 2), (40, 1), (128, 1)])
+def test_split_head_groups(cuda, product_lib, hq, hkv):
+    torch = cuda
+    d = inputs(torch, 90 + hq, [25, 7], [9000, 31], hq, hkv, gain=12.0)
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, d)
+
+
 def test_long_prompt(cuda, product_lib):
     """Many query tiles a CTA, the ring and every barrier through many phases."""
     torch = cuda
@@ -187,16 +210,20 @@ def test_lists_out_of_order(cuda, product_lib):
 
 
 def test_repeats_streams_and_graphs(cuda, product_lib):
-    """The same call gives the same bits, eagerly and from graphs of two calls replayed side by side."""
+    """The same call gives the same bits, eagerly and from graphs of several calls, split ones with a workspace each, replayed
+    side by side."""
     torch = cuda
     row = product_lib.find_row("ridgefill_attn_prefill", abi.DOMAIN_DEVICE)
     calls = []
-    for seed, n in ((59, [500, 33]), (60, [1200])):
-        d = inputs(torch, seed, n, n, 16, 2)
+    for seed, n, nk in ((59, [500, 33], [500, 33]), (60, [1200], [1200]), (61, [70], [9999]), (62, [200], [8500])):
+        d = inputs(torch, seed, n, nk, 16, 2)
         assert call(product_lib, torch, d) == abi.OK
         check(torch, d)
         ops, keep = operands(torch, d)
-        bound = product_lib.bind(row, ops, S.prefill_params(sum(n), 16, 2))
+        size = product_lib.scratch_bytes(row, ops, S.prefill_params(sum(n), 16, 2))
+        ws = torch.full((max(size, 16),), 0xFF, dtype=torch.uint8, device="cuda")
+        keep.append(ws)
+        bound = product_lib.bind(row, ops, S.prefill_params(sum(n), 16, 2), scratch=ws.data_ptr(), scratch_bytes=size)
         graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
         with torch.cuda.graph(graph, stream=stream):
             assert bound(torch.cuda.current_stream().cuda_stream) == abi.OK

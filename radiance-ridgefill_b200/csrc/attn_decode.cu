@@ -424,13 +424,46 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Plan
     }
 }
 
-constexpr int kJoinThreads = 256, kJoinFlight = 8;
+
+struct Sums {   /* four elements of a row's sum, with the maximum and the sum of weights they go by */
+    float m = kNone, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+};
+
+/* Adds pieces first, first + step, ... below n to `s`, kFlight pieces' loads in flight. */
+template <int NT, int kFlight>
+__device__ __forceinline__ void add_pieces(Sums& s, const Partial<NT>* pieces, int first, int step, int n, int row, int d) {
+    for (int i0 = first; i0 < n; i0 += kFlight * step) {
+        float pm[kFlight], pl[kFlight];
+        float4 po[kFlight];
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) {
+            const int i = i0 + k * step;
+            const Partial<NT>& x = pieces[2 * min(i, n - 1) + (i == 0 ? 1 : 0)];
+            pm[k] = i < n ? x.m[row] : kNone;
+            pl[k] = i < n ? x.l[row] : 0.f;
+            po[k] = i < n ? *(const float4*)&x.o[row][d] : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float up = s.m;
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) up = fmaxf(up, pm[k]);
+        const float f = s.m == kNone ? 0.f : exp2_approx(s.m - up);
+        s.l *= f;
+        s.o = make_float4(s.o.x * f, s.o.y * f, s.o.z * f, s.o.w * f);
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) {
+            const float w = pm[k] == kNone ? 0.f : exp2_approx(pm[k] - up);
+            s.l = fmaf(w, pl[k], s.l);
+            s.o = make_float4(fmaf(w, po[k].x, s.o.x), fmaf(w, po[k].y, s.o.y), fmaf(w, po[k].z, s.o.z), fmaf(w, po[k].w, s.o.w));
+        }
+        s.m = up;
+    }
+}
 
 /* The items the split kernel cut. The pieces of an item lie in the slots of the CTAs that own its first to last block:
  * slot 1 of the first, slot 0 of the others. A CTA joins D / p.parts elements of one query head of a sequence: groups of
- * threads, four elements a thread, take every so-many-th piece, kJoinFlight pieces' loads in flight, with a running
- * maximum of their own, and meet at the end. */
-template <int NT>
+ * threads, four elements a thread, take every so-many-th piece with a running maximum of their own, and meet at the end. */
+template <int NT, int kFlight, int kJoinThreads>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Plan p) {
     __shared__ float4 sums[kJoinThreads];
     __shared__ float2 stats[kJoinThreads];
@@ -459,40 +492,15 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Plan p) {
     if (n == 1) return;   /* written by its one CTA */
     asm volatile("griddepcontrol.wait;" ::: "memory");   /* the split kernel is done and its results are visible */
     const Partial<NT>* pieces = (const Partial<NT>*)p.partials + 2 * (int64_t)c0;
-    float m = kNone, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = group; i0 < n; i0 += kJoinFlight * groups) {
-        float pm[kJoinFlight], pl[kJoinFlight];
-        float4 po[kJoinFlight];
-#pragma unroll
-        for (int k = 0; k < kJoinFlight; ++k) {
-            const int i = i0 + k * groups;
-            const Partial<NT>& s = pieces[2 * min(i, n - 1) + (i == 0 ? 1 : 0)];
-            pm[k] = i < n ? s.m[row] : kNone;
-            pl[k] = i < n ? s.l[row] : 0.f;
-            po[k] = i < n ? *(const float4*)&s.o[row][d] : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-        float up = m;
-#pragma unroll
-        for (int k = 0; k < kJoinFlight; ++k) up = fmaxf(up, pm[k]);
-        const float f = m == kNone ? 0.f : exp2_approx(m - up);
-        l *= f;
-        acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
-#pragma unroll
-        for (int k = 0; k < kJoinFlight; ++k) {
-            const float w = pm[k] == kNone ? 0.f : exp2_approx(pm[k] - up);
-            l = fmaf(w, pl[k], l);
-            acc = make_float4(fmaf(w, po[k].x, acc.x), fmaf(w, po[k].y, acc.y), fmaf(w, po[k].z, acc.z), fmaf(w, po[k].w, acc.w));
-        }
-        m = up;
-    }
-    sums[tid] = acc;
-    stats[tid] = make_float2(m, l);
+    Sums mine;
+    add_pieces<NT, kFlight>(mine, pieces, group, groups, n, row, d);
+    sums[tid] = mine.o;
+    stats[tid] = make_float2(mine.m, mine.l);
     __syncthreads();
     if (group > 0) return;
     float top = kNone, sum = 0.f;
     for (int k = 0; k < groups; ++k) top = fmaxf(top, stats[tid + k * lanes].x);
-    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int k = 0; k < groups; ++k) {
         const float2 s = stats[tid + k * lanes];
         const float4 v = sums[tid + k * lanes];
@@ -534,18 +542,24 @@ int launch(const Plan& p, bool split, cudaStream_t s) {
     const int64_t grid = split ? p.ctas : p.g.B * p.g.n_head_kv * p.chunks;
     decode_kernel<NT><<<(unsigned)grid, kThreads, kSmem, s>>>(p);
     if (!split) return rf::launch_status();
+    const int rc = rf::launch_status();
+    if (rc != RAD_OK) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.g.B * p.g.n_head * p.parts));
-    cfg.blockDim = dim3(kJoinThreads);
+    /* Loads in flight a thread and threads a CTA, by how many pieces an item may have and how many CTAs there are. One
+     * sequence of 32,768 keys: 24.4 us with 16 loads, 26.0 with 8; of 500: 8.0 with 2, 8.9 with 16. 32 short sequences, a few
+     * pieces each: 25.1 us with CTAs so small that all run at once, 30.3 with the registers of 16 loads. 64 long ones, a dozen
+     * pieces each: 399 us with 8 loads, 404 with the small CTAs. */
+    const bool few = p.parts > 1, many_pieces = p.g.n_pages * p.g.page > 32 * kRound;
+    cfg.blockDim = dim3(few || p.narrow ? 256 : 128);
     cfg.stream = s;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    const int rc = rf::launch_status();
-    if (rc != RAD_OK) return rc;
-    if (cudaLaunchKernelEx(&cfg, join_kernel<NT>, p) != cudaSuccess) {
+    if (cudaLaunchKernelEx(&cfg, few ? (many_pieces ? join_kernel<NT, 16, 256> : join_kernel<NT, 2, 256>)
+                                     : p.narrow ? join_kernel<NT, 8, 256> : join_kernel<NT, 4, 128>, p) != cudaSuccess) {
         cudaGetLastError();
         return RAD_E_DEVICE;
     }
@@ -573,7 +587,7 @@ extern "C" int ridgefill_attn_decode_device(const RadArgs* a, RadStream s) {
     p.ctas = sh.ctas;
     p.seats = sh.seats;
     p.narrow = sh.narrow;
-    /* few heads have many pieces each: four CTAs a head share them (29 -> 26 us for one sequence of 32,768) */
+    /* few heads may have many pieces each: four CTAs a head share them (29 -> 27 us for one sequence of 32,768) */
     p.parts = p.g.B * p.g.n_head <= sh.seats ? 4 : 1;
     p.partials = sh.split ? a->scratch : nullptr;
     p.scale_log2 = p.g.scale * 1.4426950408889634f;

@@ -167,6 +167,7 @@ class Plugin:
         self.path = path
         self.lib = C.CDLL(str(path), mode=os.RTLD_LOCAL | os.RTLD_NOW)
         L = self.lib
+        self._found = None
         L.rad_plugin_abi_version.restype = C.c_uint32
         L.rad_plugin_info.restype = C.POINTER(RadPluginInfo)
         L.rad_kernel_schema_count.restype = C.c_int
@@ -213,10 +214,11 @@ class Plugin:
         return [self.lib.ridgefill_serve_at(i).contents for i in range(n)]
 
     def find_row(self, op: str, domain: int) -> RadKernelInfo | None:
-        for r in self.rows() + self.serve_rows():
-            if r.domain == domain and r.op.decode() == op:
-                return r
-        return None
+        if self._found is None:   # the tables are constant: read once
+            self._found = {}
+            for r in self.rows() + self.serve_rows():
+                self._found.setdefault((r.op.decode(), r.domain), r)
+        return self._found.get((op, domain))
 
     @staticmethod
     def args(tensors, params, scratch: int | None = None, scratch_bytes: int = 0):

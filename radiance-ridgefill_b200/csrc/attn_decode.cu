@@ -13,9 +13,9 @@
  * launch overlaps this one's run, adds the pieces of each item.
  *
  * Inside a CTA four warps take 16-key blocks in turn, each with running softmax statistics of its own, and meet at the
- * piece's end. A warp streams its blocks through its own ring in shared memory by 16-byte asynchronous copies that each
- * lane issues and reads back itself: no barrier, no bank conflict, and two to three 8 KiB halves in flight a warp (128 KiB
- * a SM; the 44 bytes a nanosecond of a SM's share of HBM at about a microsecond's latency need 44 KiB). The products are
+ * piece's end. A warp streams its blocks through its own ring in shared memory by 16-byte asynchronous copies, a
+ * whole 512-byte row an instruction: no barrier beyond the warp's own, and two to three 8 KiB halves in flight a warp
+ * (128 KiB a SM; the 49 bytes a nanosecond of a SM's share of HBM at about a microsecond's latency need 49 KiB). The products are
  * taken transposed, S^T = K Q^T and O^T = V^T P^T, so that the up to 8 query heads sharing a kv head fill the n of
  * m16n8k16 exactly:
  *   lane (r = lane / 4, c = lane % 4) holds keys r and r + 8, elements 32 j + 8 c .. + 7 of K: the A operand up to an
@@ -110,26 +110,19 @@ __device__ __forceinline__ int slot_of(const RidgeFillAttnDecode& g, const Block
     return slot >= 0 && slot < g.n_slots ? (int)slot : -1;
 }
 
-/* Lane's copies of one half (K when !values, else V) of the block whose slots the lanes 0..15 hold in `slots`. */
+/* The 16-byte chunk in whose place chunk x of a block's row i lies, so that a warp's reads below meet no bank conflict. */
+__device__ __forceinline__ constexpr int key_chunk(int i, int x) { return x ^ ((i & 1) << 2); }
+__device__ __forceinline__ constexpr int value_chunk(int i, int x) { return x ^ ((i >> 1 & 3) << 1); }
+
+/* The copies of one half (K when !values, else V) of the block whose slots the lanes 0..15 hold in `slots`: a row of 512
+ * bytes an instruction, in whole 128-byte lines. */
 __device__ __forceinline__ void fetch(const RidgeFillAttnDecode& g, const Blocks& w, int slots, bool values, uint8_t* half, int lane) {
-    const int r = lane >> 2, c = lane & 3;
-    if (!values) {
-        const int s0 = __shfl_sync(0xffffffffu, slots, r), s1 = __shfl_sync(0xffffffffu, slots, r + 8);
-        const uint16_t* p0 = w.keys + (int64_t)max(s0, 0) * g.c_slot + 8 * c;
-        const uint16_t* p1 = w.keys + (int64_t)max(s1, 0) * g.c_slot + 8 * c;
+    const uint16_t* plane = w.keys + (values ? g.c_kv : 0) + 8 * lane;
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-            rf::cp_async16_l2(half + (2 * j) * 512 + lane * 16, p0 + 32 * j, s0 >= 0 ? 16 : 0);
-            rf::cp_async16_l2(half + (2 * j + 1) * 512 + lane * 16, p1 + 32 * j, s1 >= 0 ? 16 : 0);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int s = __shfl_sync(0xffffffffu, slots, 2 * c + (i & 1) + (i >> 1) * 8);
-            const uint16_t* p = w.keys + g.c_kv + (int64_t)max(s, 0) * g.c_slot + 8 * r;
-#pragma unroll
-            for (int j = 0; j < D / 64; ++j) rf::cp_async16_l2(half + (4 * j + i) * 512 + lane * 16, p + 64 * j, s >= 0 ? 16 : 0);
-        }
+    for (int i = 0; i < kBlock; ++i) {
+        const int s = __shfl_sync(0xffffffffu, slots, i);
+        const int at = values ? value_chunk(i, lane) : key_chunk(i, lane);
+        rf::cp_async16_l2(half + i * 512 + at * 16, plane + (int64_t)max(s, 0) * g.c_slot, s >= 0 ? 16 : 0);
     }
     rf::cp_async_commit();
 }
@@ -176,16 +169,19 @@ __device__ __forceinline__ void run_piece(const Plan& p, uint8_t* smem, int b, i
         const int after = i + 2 < n ? slot_of(g, w, first + (i + 2) * kRound + (lane & 15)) : -1;
         /* scores of the block's 16 keys */
         int free_slot = at + 2 >= kRing ? at + 2 - kRing : at + 2;
+        __syncwarp();   /* every lane has read the half that lay there */
         if (i + 1 < n) fetch(g, w, next, false, ring + free_slot * kHalfBytes, lane);
         else rf::cp_async_commit();
         rf::cp_async_wait<2>();
+        __syncwarp();   /* every lane's copies have landed */
         float s[NT][4];
 #pragma unroll
         for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-        const uint8_t* kh = ring + at * kHalfBytes + lane * 16;
+        const uint8_t* kh = ring + at * kHalfBytes + r * 512;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
-            const uint4 k0 = *(const uint4*)(kh + (2 * j) * 512), k1 = *(const uint4*)(kh + (2 * j + 1) * 512);
+            const int x = key_chunk(r, 4 * j + c) * 16;   /* row r + 8 alike */
+            const uint4 k0 = *(const uint4*)(kh + x), k1 = *(const uint4*)(kh + 8 * 512 + x);
             const uint32_t a0[4] = { k0.x, k1.x, k0.y, k1.y }, a1[4] = { k0.z, k1.z, k0.w, k1.w };
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
@@ -242,15 +238,17 @@ __device__ __forceinline__ void run_piece(const Plan& p, uint8_t* smem, int b, i
         }
         /* O^T += V^T P^T */
         free_slot = at + 2 >= kRing ? at + 2 - kRing : at + 2;
+        __syncwarp();
         if (i + 1 < n) fetch(g, w, next, true, ring + free_slot * kHalfBytes, lane);
         else rf::cp_async_commit();
         rf::cp_async_wait<2>();
-        const uint8_t* vh = ring + at * kHalfBytes + lane * 16;
+        __syncwarp();
+        const uint8_t* vh = ring + at * kHalfBytes + 2 * c * 512 + value_chunk(2 * c, r) * 16;   /* keys 2c, 2c+1, 2c+8, 2c+9 alike */
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) {
             uint4 v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = *(const uint4*)(vh + (4 * j + e) * 512);
+            for (int e = 0; e < 4; ++e) v[e] = *(const uint4*)(vh + ((e & 1) + (e >> 1) * 8) * 512 + j * 128);
             const uint32_t* v0 = &v[0].x;
             const uint32_t* v1 = &v[1].x;
             const uint32_t* v2 = &v[2].x;

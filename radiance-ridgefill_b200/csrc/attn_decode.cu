@@ -122,7 +122,7 @@ __device__ __forceinline__ void fetch(const RidgeFillAttnDecode& g, const Blocks
     for (int i = 0; i < kBlock; ++i) {
         const int s = __shfl_sync(0xffffffffu, slots, i);
         const int at = values ? value_chunk(i, lane) : key_chunk(i, lane);
-        rf::cp_async16_l2(half + i * 512 + at * 16, plane + (int64_t)max(s, 0) * g.c_slot, s >= 0 ? 16 : 0);
+        rf::cp_async16(half + i * 512 + at * 16, plane + (int64_t)max(s, 0) * g.c_slot, s >= 0 ? 16 : 0);
     }
     rf::cp_async_commit();
 }
@@ -139,6 +139,14 @@ __device__ __forceinline__ void run_piece(const Plan& p, uint8_t* smem, int b, i
     const int first = from + warp * kBlock;
     const int n = first < to ? (to - first + kRound - 1) / kRound : 0;   /* this warp's blocks */
 
+    /* halves 2 i (keys) and 2 i + 1 (values) of block i go through slot (2 i) % kRing, ... of the ring, kRing - 1 ahead */
+    int cur = -1, next = -1;   /* lanes 0..15: the slots of blocks i and i + 1 */
+    if (n > 0) {
+        cur = slot_of(g, w, first + (lane & 15));
+        next = n > 1 ? slot_of(g, w, first + kRound + (lane & 15)) : -1;
+        fetch(g, w, cur, false, ring, lane);
+        fetch(g, w, cur, true, ring + kHalfBytes, lane);
+    }
     float o[NT][D / 16][4], m[NT][2], l[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -155,14 +163,6 @@ __device__ __forceinline__ void run_piece(const Plan& p, uint8_t* smem, int b, i
         const uint16_t* src = g.q + b * g.q_row + (int64_t)(hkv * p.group + h0 + h) * g.q_head + 8 * c;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) q[t][j] = h < heads ? *(const uint4*)(src + 32 * j) : make_uint4(0u, 0u, 0u, 0u);
-    }
-    /* halves 2 i (keys) and 2 i + 1 (values) of block i go through slot (2 i) % kRing, ... of the ring, kRing - 1 ahead */
-    int cur = -1, next = -1;   /* lanes 0..15: the slots of blocks i and i + 1 */
-    if (n > 0) {
-        cur = slot_of(g, w, first + (lane & 15));
-        next = n > 1 ? slot_of(g, w, first + kRound + (lane & 15)) : -1;
-        fetch(g, w, cur, false, ring, lane);
-        fetch(g, w, cur, true, ring + kHalfBytes, lane);
     }
     int at = 0;   /* ring slot of the current half */
     for (int i = 0; i < n; ++i) {
@@ -374,8 +374,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Plan
         return;
     }
     const int B = (int)g.B;
-    int total = 0;
-    for (int i = lane; i < B; i += 32) total += units_of(g, i);
+    const int mine = lane < B ? units_of(g, lane) : 0;   /* the first 32 sequences', a lane each */
+    int total = mine;
+    for (int i = 32 + lane; i < B; i += 32) total += units_of(g, i);
     total = warp_sum(total) * items;
     if (total == 0) return;
     const Spans spans(total, p.seats, p.narrow);
@@ -385,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Plan
     /* the sequence holding unit u: blocks of 32 sequences, then an inclusive scan inside the block */
     int b = 0, base = 0;
     for (;; b += 32) {
-        int sum = b + lane < B ? units_of(g, b + lane) * items : 0;
+        int sum = b == 0 ? mine * items : b + lane < B ? units_of(g, b + lane) * items : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int up = __shfl_up_sync(0xffffffffu, sum, o);

@@ -113,10 +113,6 @@ __device__ __forceinline__ void c_to_a(uint32_t (&a)[4], const float (&lo)[4], c
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, int src_bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(saddr(dst)), "l"(src), "r"(src_bytes) : "memory");
 }
-/* cp_async16 that also brings the 256 bytes around its source into L2: for a source whose neighbours are read next. */
-__device__ __forceinline__ void cp_async16_l2(void* dst, const void* src, int src_bytes) {
-    asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(saddr(dst)), "l"(src), "r"(src_bytes) : "memory");
-}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }

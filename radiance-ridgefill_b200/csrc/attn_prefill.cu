@@ -476,7 +476,9 @@ __device__ void soften(const Plan& p, Shared& s, uint32_t tmem, int warp, int la
     const float sl2 = p.scale_log2;
     for (;;) {
         const Item it = items.next(lane);
-        if (it.rows < 0) return;
+        /* the two warps of these rows meet once a query tile and once a key tile, and leave together: when a wait gave up
+         * neither is left at a barrier */
+        if (rf::bar_any(1 + quarter, 64, it.rows < 0)) return;
         if (it.tiles == 0) continue;
         const int limit = it.limit + min(token, max(it.rows - 1, 0));   /* this row's last key */
         float m = kNone, l0 = 0.f, l1 = 0.f;
@@ -507,7 +509,7 @@ __device__ void soften(const Plan& p, Shared& s, uint32_t tmem, int warp, int la
             }
             const float own = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
             s.top[tile & 1][half][row] = own;
-            /* both warps have read their scores, so that P may take their place; they leave together when a wait gave up */
+            /* both warps have read their scores, so that P may take their place */
             if (rf::bar_any(1 + quarter, 64, !ok)) return;
             const float mt = fmaxf(own, s.top[tile & 1][half ^ 1][row]) * sl2;
             const bool grow = mt > m + kGrow;
@@ -810,7 +812,7 @@ bool head_map(CUtensorMap* map, const uint16_t* base, int64_t T, int64_t heads, 
     PFN_cuTensorMapEncodeTiled_v12000 enc = rf::tensor_map_encoder();
     if (!enc) return false;
     if (heads == 1) head_stride = D;
-    if (T == 1) row_stride = heads * head_stride;
+    if (T == 1) row_stride = heads * D;
     const cuuint64_t dims[3] = { (cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)T };
     const cuuint64_t strides[2] = { (cuuint64_t)head_stride * 2, (cuuint64_t)row_stride * 2 };
     const cuuint32_t box[3] = { 64, (cuuint32_t)heads_box, (cuuint32_t)rows_box };

@@ -129,6 +129,31 @@ def test_strides(cuda, product_lib):
     check(torch, dict(d, lens=torch.tensor([50 * 16] * B)), 0.11)
 
 
+def test_head_major_cache(cuda, product_lib):
+    """The cache kept as [Hkv, 2, slots, D], o and q a head after the other."""
+    torch = cuda
+    d = inputs(torch, 50, [700, 33, 128], 12, 3, 16)
+    d["cache"] = d["cache"].permute(2, 0, 1, 3).contiguous().permute(1, 2, 0, 3)
+    d["q"] = d["q"].transpose(0, 1).contiguous().transpose(0, 1)
+    d["o"] = torch.full((12, 3, D), 7.0, dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+    assert call(product_lib, d) == abi.OK
+    check(torch, d)
+
+
+def test_empty_pool_and_table(cuda, product_lib):
+    """No slot in the pool, or no page in the table: every row is zero."""
+    torch = cuda
+    d = inputs(torch, 51, [300, 40], 8, 2, 16)
+    empty = dict(d, cache=d["cache"][:, :0], o=d["o"].clone())
+    ops = [H.dev(d["q"]), abi.tensor(abi.BF16, (2, 0, 2, D), d["cache"].data_ptr(), (0, 512, 256, 1)), H.dev(d["table"]), H.dev(d["lens"]),
+           H.dev(empty["o"])]
+    assert H.launch(product_lib, "ridgefill_attn_decode", ops, S.decode_params(2, 8, 2, 16)) == abi.OK
+    assert (empty["o"] == 0).all()
+    ops = [H.dev(d["q"]), H.dev(d["cache"]), abi.tensor(abi.I32, (2, 0), d["table"].data_ptr()), H.dev(d["lens"]), H.dev(d["o"])]
+    assert H.launch(product_lib, "ridgefill_attn_decode", ops, S.decode_params(2, 8, 2, 16)) == abi.OK
+    assert (d["o"] == 0).all()
+
+
 def test_pages_outside_the_pool(cuda, product_lib):
     """Keys on pages outside the pool are left out; a sequence that only has such is zero. The pool's last page may be
     cut short."""

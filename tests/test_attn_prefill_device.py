@@ -166,6 +166,30 @@ def test_strides_and_scale(cuda, product_lib):
     check(torch, d)
 
 
+@pytest.mark.parametrize("T", [1, 45, 260])
+def test_head_major_operands(cuda, product_lib, T):
+    """q, k, v and o kept a head after the other ([heads, rows, D] seen as [rows, heads, D]), o larger than its rows."""
+    torch = cuda
+    d = inputs(torch, 70 + T, [T], [T], 12, 3)
+    for name in ("q", "k", "v"):
+        d[name] = d[name].transpose(0, 1).contiguous().transpose(0, 1)
+    whole = torch.full((12, T + 2, D), 7.0, dtype=torch.bfloat16, device="cuda")
+    d["o"] = whole[:, 1:T + 1].transpose(0, 1)
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, d)
+    assert (whole[:, 0] == 7.0).all() and (whole[:, T + 1] == 7.0).all()
+
+
+def test_in_place(cuda, product_lib):
+    """o may be q itself."""
+    torch = cuda
+    d = inputs(torch, 75, [300, 41], [300, 41], 16, 2)
+    q = d["q"].clone()
+    d["o"] = d["q"]
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, dict(d, q=q))
+
+
 def test_nan_stays_in_its_sequence(cuda, product_lib):
     """NaN and infinities in one sequence's q, k and v reach no row of another, nor rows 128 or more before them; keys'
     NaN reach no earlier row at all."""

@@ -459,6 +459,12 @@ __device__ __forceinline__ void add_pieces(Sums& s, const Partial<NT>* pieces, i
     }
 }
 
+/* A join CTA with nothing to add leaves at once, but for one: the join's end is what the stream's next kernel waits for, and
+ * it must not come before the split's. */
+__device__ __forceinline__ void nothing_to_join() {
+    if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 /* The items the split kernel cut. The pieces of an item lie in the slots of the CTAs that own its first to last block:
  * slot 1 of the first, slot 0 of the others. A CTA joins D / p.parts elements of one query head of a sequence: groups of
  * threads, four elements a thread, take every so-many-th piece with a running maximum of their own, and meet at the end. */
@@ -477,7 +483,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Plan p) {
     const int units = units_of(g, b);
     if (units == 0) {   /* no key: zeros */
         if (group == 0) *(uint2*)out = make_uint2(0u, 0u);
-        return;
+        return nothing_to_join();
     }
     int total = 0, before = 0;
     for (int i = lane; i < B; i += 32) {
@@ -488,7 +494,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Plan p) {
     const Spans spans(warp_sum(total) * items, p.seats, p.narrow);
     const int start = warp_sum(before) * items + it * units;
     const int c0 = spans.owner(start + kStart), n = spans.owner(start + units - 1) - c0 + 1;
-    if (n == 1) return;   /* written by its one CTA */
+    if (n == 1) return nothing_to_join();   /* written by its one CTA */
     asm volatile("griddepcontrol.wait;" ::: "memory");   /* the split kernel is done and its results are visible */
     const Partial<NT>* pieces = (const Partial<NT>*)p.partials + 2 * (int64_t)c0;
     Sums mine;
@@ -578,8 +584,9 @@ extern "C" int ridgefill_attn_decode_device(const RadArgs* a, RadStream s) {
     if (rc != RAD_OK) return rc;
     if (p.g.B == 0) return RAD_OK;
     /* grids, and the units of all items, in 32 bits */
-    if (p.g.B > 0x7fffffffLL / p.g.n_head || p.g.B * p.g.n_head * (p.g.n_pages * p.g.page / kBlock + 1 + kStart) > 0x7fffffffLL) return RAD_E_SHAPE;
+    if (p.g.B > 0x7fffffffLL / p.g.n_head) return RAD_E_SHAPE;
     const Shape sh = shape_of(p.g);
+    if (p.g.B * p.g.n_head_kv * sh.chunks * (p.g.n_pages * p.g.page / kBlock + 1 + kStart) > 0x7fffffffLL) return RAD_E_SHAPE;
     if (sh.split && (!a->scratch || a->scratch_bytes < sh.bytes || (uintptr_t)a->scratch % 16)) return RAD_E_INVAL;
     p.group = (int)(p.g.n_head / p.g.n_head_kv);
     p.chunks = sh.chunks;

@@ -727,6 +727,12 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     if (warp == 13) rf::tmem_free_pair<kTmemCols>(tmem);
 }
 
+/* A join CTA with nothing to add leaves at once, but for one: the join's end is what the stream's next kernel waits for, and
+ * it must not come before the split's. */
+__device__ __forceinline__ void nothing_to_join() {
+    if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 constexpr int kJoinCols = 64, kJoinParts = D / kJoinCols;
 
 /* The query tiles that the split cut, and those without a key (zeros): a CTA joins kJoinCols columns of a CTA's share of
@@ -749,18 +755,18 @@ __global__ void __launch_bounds__(kTileM) join_kernel(const Plan p) {
         units += warp_sum(depth);
         return false;
     });
-    if (tiles < 0) return;   /* fewer query tiles than the grid has places for */
+    if (tiles < 0) return nothing_to_join();   /* fewer query tiles than the grid has places for */
     const int token = row / p.group;
     uint16_t* out = g.o + (int64_t)(it.q0 + token) * g.o_row + (int64_t)(head * p.group + row - token * p.group) * g.o_head + part * kJoinCols;
     const bool live = token < it.rows;
     if (tiles == 0) {
         if (live)
             for (int c = 0; c < kJoinCols / 8; ++c) *(uint4*)(out + 8 * c) = make_uint4(0u, 0u, 0u, 0u);
-        return;
+        return nothing_to_join();
     }
     const Spans spans(units * heads, p.pairs);
     const int c0 = spans.owner(start), n = spans.owner(start + tiles - 1) - c0 + 1;
-    if (n == 1) return;   /* written by its one pair */
+    if (n == 1) return nothing_to_join();   /* written by its one pair */
     asm volatile("griddepcontrol.wait;" ::: "memory");   /* the split is done and its results are visible */
     auto piece = [&](int i) -> const Partial& { return ((const Partial*)p.partials)[((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * 2 + rank]; };
     float top = kNone, sum = 0.f, acc[kJoinCols];
@@ -800,7 +806,8 @@ Shape shape_of(const RidgeFillAttnPrefill& g) {
     s.tokens = kTileM / s.group;
     s.items = (g.T / (2 * s.tokens) + g.n_seq) * g.n_head_kv;
     s.pairs = rf::sm_count() / 2;
-    s.split = g.Tk >= kLongKeys && s.items <= 2 * s.pairs;
+    /* the split counts key tiles in 32 bits, whatever cu_seqlens and cu_keys hold: sequences that overlap too */
+    s.split = g.Tk >= kLongKeys && s.items <= 2 * s.pairs && g.n_seq * s.items * (g.Tk / kTileN + 1) <= 0x7fffffffLL;
     s.bytes = s.split ? (int64_t)s.pairs * 4 * (int64_t)sizeof(Partial) : 0;
     return s;
 }
@@ -840,7 +847,7 @@ extern "C" int ridgefill_attn_prefill_device(const RadArgs* a, RadStream s) {
     const RidgeFillAttnPrefill& g = p.g;
     if (g.T == 0 || g.n_seq == 0) return RAD_OK;
     const Shape sh = shape_of(g);
-    if (sh.items > 0x3fffffffLL || (sh.split && sh.items * (g.Tk / kTileN + 1) > 0x7fffffffLL)) return RAD_E_SHAPE;
+    if (sh.items > 0x3fffffffLL) return RAD_E_SHAPE;
     if (sh.split && (!a->scratch || a->scratch_bytes < sh.bytes || (uintptr_t)a->scratch % 16)) return RAD_E_INVAL;
     p.group = sh.group;
     p.tokens = sh.tokens;

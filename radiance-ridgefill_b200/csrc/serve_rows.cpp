@@ -217,11 +217,11 @@ extern "C" int ridgefill_attn_decode_parse(const RadArgs* a, RidgeFillAttnDecode
     if (!scale_of(a, D, true, &g->scale)) return RAD_E_INVAL;
     if (Q->dtype != RAD_BF16 || C->dtype != RAD_BF16 || T->dtype != RAD_I32 || L->dtype != RAD_I32 || O->dtype != RAD_BF16)
         return RAD_E_DTYPE;
-    if (B < 0 || h <= 0 || hkv <= 0 || page <= 0 || page > 1 << 20) return RAD_E_SHAPE;
+    if (B < 0 || B > 0x7fffffffLL || h <= 0 || hkv <= 0 || page <= 0 || page > 1 << 20) return RAD_E_SHAPE;
     if (h % hkv != 0 || h / hkv > 128) return RAD_E_UNSUPPORTED;
     if (!is(Q, { B, h, D }) || !is(O, { B, h, D }) || !is(L, { B })) return RAD_E_SHAPE;
     if (C->rank != 4 || !is(C, { 2, C->shape[1], hkv, D }) || C->shape[1] < 0 || C->shape[1] > 0x7fffffffLL) return RAD_E_SHAPE;
-    if (T->rank != 2 || T->shape[0] != B || T->shape[1] < 0 || T->shape[1] * page > 0x7fffff00LL) return RAD_E_SHAPE;
+    if (T->rank != 2 || T->shape[0] != B || T->shape[1] < 0 || T->shape[1] > 0x7fffff00LL / page) return RAD_E_SHAPE;
     if (!word_rows(Q) || !word_rows(C) || !word_rows(O) || !packed(L) || (T->shape[1] > 1 && T->stride[1] != 1))
         return RAD_E_STRIDE;
     g->q = (const uint16_t*)Q->data;

@@ -236,3 +236,33 @@ def test_repeats_streams_and_graphs(cuda, product_lib):
         torch.cuda.synchronize()
         for d, want, _, _, _ in calls:
             assert torch.equal(d["o"], want)
+
+
+@pytest.mark.parametrize("lens", [[16] * 4, [60] * 300, [12, 0, 3], [2000, 7]])
+def test_next_kernel_sees_the_answer(cuda, product_lib, lens):
+    """What follows the call on its stream, or in its graph, comes after all of it: also where no item needs the join, whose
+    launch overlaps the first kernel's run."""
+    torch = cuda
+    d = inputs(torch, 50, lens, 16, 2, 16, width=64)
+    row = product_lib.find_row("ridgefill_attn_decode", abi.DOMAIN_DEVICE)
+    params, ops = S.decode_params(len(lens), 16, 2, 16), [H.dev(d[n]) for n in ("q", "cache", "table", "lens", "o")]
+    n = product_lib.scratch_bytes(row, ops, params)
+    ws = torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")
+    bound = product_lib.bind(row, ops, params, scratch=ws.data_ptr(), scratch_bytes=n)
+    stream, graph, seen = torch.cuda.Stream(), torch.cuda.CUDAGraph(), torch.empty_like(d["o"])
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        assert bound(torch.cuda.current_stream().cuda_stream) == abi.OK
+        seen.copy_(d["o"])
+        d["o"].fill_(7.0)
+    with torch.cuda.stream(stream):
+        for _ in range(20):
+            graph.replay()
+            stream.synchronize()
+            check(torch, dict(d, o=seen))
+        for _ in range(20):
+            assert bound(stream.cuda_stream) == abi.OK
+            seen.copy_(d["o"])
+            d["o"].fill_(7.0)
+            stream.synchronize()
+            check(torch, dict(d, o=seen))

@@ -263,3 +263,49 @@ def test_repeats_streams_and_graphs(cuda, product_lib):
         for d, want, *_ in calls:
             assert torch.equal(d["o"], want)
     assert product_lib.lib.ridgefill_device_error(1) == 0
+
+
+@pytest.mark.parametrize("nq,nk", [([16] * 3, [512] * 3), ([5, 16], [0, 512]), ([200], [8192])])
+def test_next_kernel_sees_the_answer(cuda, product_lib, nq, nk):
+    """What follows a split call on its stream, or in its graph, comes after all of it: also where every span is a whole query
+    tile, so that the join, whose launch overlaps the split's run, has nothing to add."""
+    torch = cuda
+    d = inputs(torch, 63, nq, nk, 8, 1)
+    more = 9000 - d["k"].shape[0]   # rows behind the last sequence: the call is split by the operands' extent
+    if more > 0:
+        d["k"], d["v"] = (torch.cat([d[x], torch.full((more, 1, D), float("nan"), dtype=d[x].dtype, device="cuda")]) for x in "kv")
+    ops, keep = operands(torch, d)
+    row, params = product_lib.find_row("ridgefill_attn_prefill", abi.DOMAIN_DEVICE), S.prefill_params(sum(nq), 8, 1)
+    n = product_lib.scratch_bytes(row, ops, params)
+    assert n > 0
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    bound = product_lib.bind(row, ops, params, scratch=ws.data_ptr(), scratch_bytes=n)
+    stream, graph, seen = torch.cuda.Stream(), torch.cuda.CUDAGraph(), torch.empty_like(d["o"])
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        assert bound(torch.cuda.current_stream().cuda_stream) == abi.OK
+        seen.copy_(d["o"])
+        d["o"].fill_(7.0)
+    with torch.cuda.stream(stream):
+        for _ in range(20):
+            graph.replay()
+            stream.synchronize()
+            check(torch, dict(d, o=seen))
+        for _ in range(20):
+            assert bound(stream.cuda_stream) == abi.OK
+            seen.copy_(d["o"])
+            d["o"].fill_(7.0)
+            stream.synchronize()
+            check(torch, dict(d, o=seen))
+
+
+def test_lists_that_overlap(cuda, product_lib):
+    """Sequences that share rows (a list that falls and rises again) read and write in range, and the rows that only the first
+    one holds are its own."""
+    torch = cuda
+    d = inputs(torch, 64, [300], [9000], 8, 2)
+    d["cu_q"], d["cu_k"] = [0, 200, 100, 300], [0, 9000, 0, 8900]   # rows 0 .. 199, none, and rows 100 .. 299
+    assert call(product_lib, torch, d) == abi.OK
+    o, bound, _ = S.prefill_reference(torch, d["q"], d["k"], d["v"], [0, 200], [0, 9000])
+    assert ((d["o"][:100].double() - o[:100]).abs() <= bound[:100]).all()
+    assert product_lib.lib.ridgefill_device_error(1) == 0

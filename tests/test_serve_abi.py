@@ -137,6 +137,9 @@ DECODE = [
     (abi.E_SHAPE, dict(kv_cache=T(abi.BF16, [2, 400, 1, 256])), {}),
     (abi.E_SHAPE, dict(block_table=T(abi.I32, [2, 5])), {}),
     (abi.E_SHAPE, dict(block_table=T(abi.I32, [3, 1 << 28])), {}),                         # keys past 32 bits
+    (abi.E_SHAPE, dict(block_table=T(abi.I32, [3, 1 << 44])), dict(page=1 << 20)),         # and past 64
+    (abi.E_SHAPE, dict(q=T(abi.BF16, [1 << 31, 16, 256]), o=T(abi.BF16, [1 << 31, 16, 256]), kv_lens=T(abi.I32, [1 << 31]),
+                       block_table=T(abi.I32, [1 << 31, 5])), dict(M=1 << 31)),
     (abi.E_SHAPE, dict(o=T(abi.BF16, [3, 16, 128])), {}),
     (abi.E_STRIDE, dict(block_table=T(abi.I32, [3, 5], [10, 2])), {}),
     (abi.E_STRIDE, dict(kv_lens=T(abi.I32, [3], [2])), {}),

@@ -640,7 +640,9 @@ __device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, u
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int x = 8 * (v & 3) + 2 * e;
-                    w[e] = pack(__uint_as_float(o[v >> 2][x]) * inv, __uint_as_float(o[v >> 2][x + 1]) * inv);
+                    float lo, hi;
+                    rf::mul2_rn(lo, hi, __uint_as_float(o[v >> 2][x]), __uint_as_float(o[v >> 2][x + 1]), inv, inv);
+                    w[e] = pack(lo, hi);
                 }
                 *(uint4*)(tile + lane * 128 + ((v ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             }

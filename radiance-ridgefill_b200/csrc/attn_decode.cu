@@ -22,6 +22,11 @@
  *   order of the contracted elements that Q shares; P^T goes from accumulators to the B operand by movmatrix; V^T's A
  *   operand pairs the keys 2c, 2c+1, 2c+8, 2c+9 of elements 64 j + 8 r .. + 7 by byte permutes, and the accumulators
  *   come out as eight consecutive elements a lane and head.
+ *
+ * Measured, 16 query heads over 2 kv heads, replayed from a graph: 64 sequences of 1 to 32,768 keys 338 us (6.58 TB/s, the
+ * measured copy rate), one of 32,768 keys 21.7 us (67 MB: 10.3 us at that rate; the rest is the launch and the lengths',
+ * tables' and first rows' latency, about 5 us, the warps' meeting, 2, and the join, 3.5), 32 of 256 to 2,038 keys 22.7 us
+ * (77 MB), one of 500 keys 7.2 us.
  */
 #include <cuda_bf16.h>
 
@@ -330,7 +335,7 @@ __device__ __forceinline__ void run_piece(const Plan& p, uint8_t* smem, int b, i
 /* The units cut into spans, CTA i taking span i. `seats` CTAs run at a time.
  * With few units: as many CTAs as have one for each of their warps, at most one a seat, equal spans.
  * From kLong units a seat on: SMs do not get equal shares of the memory's rate, so equal spans leave some idle at the
- * end (13 % of the SMs' time at 64 sequences of up to 32,768). One wide span a seat takes 4/5 of the units, and four
+ * end (64 sequences of up to 32,768: 412 us against 456 when this was chosen, 338 now). One wide span a seat takes 4/5 of the units, and four
  * times as many narrow ones follow, which the hardware gives to whichever seat comes free. */
 constexpr int kLong = 128, kNarrowPerSeat = 4;
 struct Spans {
@@ -551,10 +556,11 @@ int launch(const Plan& p, bool split, cudaStream_t s) {
     if (rc != RAD_OK) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.g.B * p.g.n_head * p.parts));
-    /* Loads in flight a thread and threads a CTA, by how many pieces an item may have and how many CTAs there are. One
-     * sequence of 32,768 keys: 24.4 us with 16 loads, 26.0 with 8; of 500: 8.0 with 2, 8.9 with 16. 32 short sequences, a few
-     * pieces each: 25.1 us with CTAs so small that all run at once, 30.3 with the registers of 16 loads. 64 long ones, a dozen
-     * pieces each: 399 us with 8 loads, 404 with the small CTAs. */
+    /* Loads in flight a thread and threads a CTA, by how many pieces an item may have and how many CTAs there are. What a
+     * whole call took beside the split as it was then (it takes 2 to 60 us less now, the join the same): one sequence of
+     * 32,768 keys 24.4 us with 16 loads, 26.0 with 8; of 500: 8.0 with 2, 8.9 with 16. 32 short sequences, a few pieces each:
+     * 25.1 us with CTAs so small that all run at once, 30.3 with the registers of 16 loads. 64 long ones, a dozen pieces each:
+     * 399 us with 8 loads, 404 with the small CTAs. */
     const bool few = p.parts > 1, many_pieces = p.g.n_pages * p.g.page > 32 * kRound;
     cfg.blockDim = dim3(few || p.narrow ? 256 : 128);
     cfg.stream = s;
@@ -593,7 +599,7 @@ extern "C" int ridgefill_attn_decode_device(const RadArgs* a, RadStream s) {
     p.ctas = sh.ctas;
     p.seats = sh.seats;
     p.narrow = sh.narrow;
-    /* few heads may have many pieces each: four CTAs a head share them (29 -> 27 us for one sequence of 32,768) */
+    /* few heads may have many pieces each: four CTAs a head share them (one sequence of 32,768: 27 us against 29 with one, when the split took 6 us more) */
     p.parts = p.g.B * p.g.n_head <= sh.seats ? 4 : 1;
     p.partials = sh.split ? a->scratch : nullptr;
     p.scale_log2 = p.g.scale * 1.4426950408889634f;

@@ -9,7 +9,7 @@
  * so a warp's load covers four rows in whole 128-byte lines); the two sums take three shuffles each. All of a lane's
  * words are loaded before the first is used. Loads and stores go through L2 alone, without the streaming hint, which cost
  * 3 % (169.8 -> 164.8 us at 256 rows of 32 heads). Four warps a CTA: 161 us, 6.70 TB/s, the measured copy rate and a little
- * more; 28.9 us at 27 rows of 48 heads (5.91 TB/s), 2.7 us at one row of 32.
+ * more; 28.9 us at 27 rows of 48 heads (5.91 TB/s), 2.9 us at one row of 32.
  */
 #include <cuda_bf16.h>
 

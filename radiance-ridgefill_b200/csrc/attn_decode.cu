@@ -23,10 +23,10 @@
  *   operand pairs the keys 2c, 2c+1, 2c+8, 2c+9 of elements 64 j + 8 r .. + 7 by byte permutes, and the accumulators
  *   come out as eight consecutive elements a lane and head.
  *
- * Measured, 16 query heads over 2 kv heads, replayed from a graph: 64 sequences of 1 to 32,768 keys 338 us (6.58 TB/s, the
- * measured copy rate), one of 32,768 keys 21.7 us (67 MB: 10.3 us at that rate; the rest is the launch and the lengths',
- * tables' and first rows' latency, about 5 us, the warps' meeting, 2, and the join, 3.5), 32 of 256 to 2,038 keys 22.7 us
- * (77 MB), one of 500 keys 7.2 us.
+ * Measured, 16 query heads over 2 kv heads, replayed from a graph: 64 sequences of 1 to 32,768 keys 335 us (6.64 TB/s, the
+ * measured copy rate), one of 32,768 keys 19.0 us (67 MB: 10.3 us at that rate; the rest is the lengths' and the tables' way
+ * from memory, 2.5 us, the first and last rows' ramp, 2, the warps' meeting, 1, and the join, 3), 32 of 256 to 2,038 keys
+ * 20.7 us (77 MB), one of 500 keys 6.3 us.
  */
 #include <cuda_bf16.h>
 
@@ -52,7 +52,7 @@ constexpr float kNone = -INFINITY;
 template <int NT>
 struct Partial {                                    /* one piece's result */
     float o[8 * NT][D];
-    float m[8 * NT], l[8 * NT];                     /* maximum (log2 units) and sum of 2^(s - m) */
+    float2 ml[8 * NT];                              /* maximum (log2 units) and sum of 2^(s - m) */
 };
 
 struct Plan {
@@ -60,6 +60,7 @@ struct Plan {
     int group, chunks;      /* query heads a kv head; items a kv head (group / heads of an item, rounded up) */
     int ctas, seats;        /* CTAs of the split kernel; how many of them run at a time */
     bool narrow;            /* its grid has CTAs for narrow spans */
+    int page_shift;         /* page as a power of two; -1: it is none */
     int parts;              /* CTAs a query head's join */
     void* partials;         /* [ctas][2] Partial; null: one CTA an item, nothing to join */
     float scale_log2;
@@ -105,12 +106,13 @@ struct Blocks {
     const uint16_t* keys;      /* cache plane 0 at the item's kv head */
     int len;                   /* the sequence's keys */
     const int32_t* table;      /* its pages */
+    int page_shift;            /* as Plan's: a division is 100 cycles before a piece's first row */
 };
 
 /* The slot of key `j` (-1: past the sequence, or outside the pool), by the lane that owns it. */
 __device__ __forceinline__ int slot_of(const RidgeFillAttnDecode& g, const Blocks& w, int j) {
     if (j >= w.len) return -1;
-    const int page = (int)g.page, n = j / page;
+    const int page = (int)g.page, n = w.page_shift >= 0 ? j >> w.page_shift : j / page;
     const int64_t slot = (int64_t)w.table[n] * page + (j - n * page);
     return slot >= 0 && slot < g.n_slots ? (int)slot : -1;
 }
@@ -132,6 +134,9 @@ __device__ __forceinline__ void fetch(const RidgeFillAttnDecode& g, const Blocks
     rf::cp_async_commit();
 }
 
+/* The 16-byte chunk in whose place chunk x of head row h lies where the warps' results meet: lanes write four heads at once. */
+__device__ __forceinline__ constexpr int sum_chunk(int h, int x) { return x ^ (h >> 1 & 1) ^ (h & 4); }
+
 /* A piece's keys [from, to) of item (b, kv head, first query head h0, heads), by the whole CTA; its result to the
  * output (`out`) or to `part`. */
 template <int NT>
@@ -140,7 +145,7 @@ __device__ __forceinline__ void run_piece(const Plan& p, uint8_t* smem, int b, i
     const RidgeFillAttnDecode& g = p.g;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
     uint8_t* ring = smem + warp * kRing * kHalfBytes;
-    const Blocks w = { g.cache + hkv * g.c_head, length_of(g, b), g.table + b * g.t_row };
+    const Blocks w = { g.cache + hkv * g.c_head, length_of(g, b), g.table + b * g.t_row, p.page_shift };
     const int first = from + warp * kBlock;
     const int n = first < to ? (to - first + kRound - 1) / kRound : 0;   /* this warp's blocks */
 
@@ -288,15 +293,14 @@ __device__ __forceinline__ void run_piece(const Plan& p, uint8_t* smem, int b, i
             for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             const int h = 8 * t + 2 * c + e;
             if (r == 0) {
-                mine[warp].m[h] = m[t][e];
-                mine[warp].l[h] = sum;
+                mine[warp].ml[h] = make_float2(m[t][e], sum);
             }
             /* elements 64 j + 8 r .. + 7 of head h: tiles 4 j .. 4 j + 3, two elements each */
 #pragma unroll
             for (int j = 0; j < D / 64; ++j)
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf)
-                    *(float4*)&mine[warp].o[h][64 * j + 8 * r + 4 * hf] =
+                    *(float4*)&mine[warp].o[h][4 * sum_chunk(h, 16 * j + 2 * r + hf)] =
                         make_float4(o[t][4 * j + 2 * hf][e], o[t][4 * j + 2 * hf][2 + e], o[t][4 * j + 2 * hf + 1][e],
                                     o[t][4 * j + 2 * hf + 1][2 + e]);
         }
@@ -305,13 +309,14 @@ __device__ __forceinline__ void run_piece(const Plan& p, uint8_t* smem, int b, i
         const int h = x / (D / 4), d = (x % (D / 4)) * 4;
         float top = kNone, sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < kWarps; ++i) top = fmaxf(top, mine[i].m[h]);
+        for (int i = 0; i < kWarps; ++i) top = fmaxf(top, mine[i].ml[h].x);
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < kWarps; ++i) {
-            const float f = mine[i].m[h] == kNone ? 0.f : exp2_approx(mine[i].m[h] - top);
-            const float4 v = *(const float4*)&mine[i].o[h][d];
-            sum = fmaf(f, mine[i].l[h], sum);
+            const float2 ml = mine[i].ml[h];
+            const float f = ml.x == kNone ? 0.f : exp2_approx(ml.x - top);
+            const float4 v = *(const float4*)&mine[i].o[h][4 * sum_chunk(h, d / 4)];
+            sum = fmaf(f, ml.y, sum);
             acc.x = fmaf(f, v.x, acc.x);
             acc.y = fmaf(f, v.y, acc.y);
             acc.z = fmaf(f, v.z, acc.z);
@@ -319,10 +324,7 @@ __device__ __forceinline__ void run_piece(const Plan& p, uint8_t* smem, int b, i
         }
         if (part) {
             *(float4*)&part->o[h][d] = acc;
-            if (d == 0) {
-                part->m[h] = top;
-                part->l[h] = sum;
-            }
+            if (d == 0) part->ml[h] = make_float2(top, sum);
         } else {
             const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);   /* no key: zeros; a NaN stays one */
             *(uint2*)(g.o + b * g.o_row + (int64_t)(hkv * p.group + h0 + h) * g.o_head + d) =
@@ -349,7 +351,7 @@ struct Spans {
             n = min((total + kWarps - 1) / kWarps, seats);
         }
         const int rest = total - n_wide * wide;
-        each = rest / n;
+        each = (int)((uint32_t)rest / (uint32_t)n);
         extra = rest - each * n;
     }
     __device__ __forceinline__ int ctas() const { return n_wide + n; }
@@ -379,6 +381,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Plan
         return;
     }
     const int B = (int)g.B;
+    {   /* the tables' lines on their way to L2 while the lengths come (32 short sequences: 20.9 us against 21.5) */
+        const int lines = (int)((g.n_pages + 31) / 32);
+        const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+        if (i < (int64_t)B * lines) {
+            const int b = (int)((uint32_t)i / (uint32_t)lines), n = (int)i - b * lines;
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(g.table + b * g.t_row + 32 * n));
+        }
+    }
     const int mine = lane < B ? units_of(g, lane) : 0;   /* the first 32 sequences', a lane each */
     int total = mine;
     for (int i = 32 + lane; i < B; i += 32) total += units_of(g, i);
@@ -413,11 +423,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Plan
         if (units > 0) {
             int rest = u - base;   /* of this sequence's units * items */
             while (rest < units * items && u < end) {
-                const int it = rest / units, h0 = it % per_kv * 8 * NT;
+                const int it = (int)((uint32_t)rest / (uint32_t)units), kv = per_kv == 1 ? it : it / per_kv, h0 = (it - kv * per_kv) * 8 * NT;
                 const int u0 = rest - it * units, n = min(units - u0, end - u), len = length_of(g, b);
                 const int first = max(u0 - kStart, 0), last = u0 + n - kStart;   /* blocks; none: the item begins in the next span */
                 if (last > 0)
-                    run_piece<NT>(p, smem, b, it / per_kv, h0, min(8 * NT, p.group - h0), first * kBlock, min(last * kBlock, len),
+                    run_piece<NT>(p, smem, b, kv, h0, min(8 * NT, p.group - h0), first * kBlock, min(last * kBlock, len),
                                   first == 0 && u0 + n == units ? nullptr : slots + (first > 0 ? 0 : 1));
                 u += n;
                 rest += n;
@@ -438,26 +448,25 @@ struct Sums {   /* four elements of a row's sum, with the maximum and the sum of
 template <int NT, int kFlight>
 __device__ __forceinline__ void add_pieces(Sums& s, const Partial<NT>* pieces, int first, int step, int n, int row, int d) {
     for (int i0 = first; i0 < n; i0 += kFlight * step) {
-        float pm[kFlight], pl[kFlight];
+        float2 ml[kFlight];
         float4 po[kFlight];
 #pragma unroll
         for (int k = 0; k < kFlight; ++k) {
             const int i = i0 + k * step;
             const Partial<NT>& x = pieces[2 * min(i, n - 1) + (i == 0 ? 1 : 0)];
-            pm[k] = i < n ? x.m[row] : kNone;
-            pl[k] = i < n ? x.l[row] : 0.f;
+            ml[k] = i < n ? x.ml[row] : make_float2(kNone, 0.f);
             po[k] = i < n ? *(const float4*)&x.o[row][d] : make_float4(0.f, 0.f, 0.f, 0.f);
         }
         float up = s.m;
 #pragma unroll
-        for (int k = 0; k < kFlight; ++k) up = fmaxf(up, pm[k]);
+        for (int k = 0; k < kFlight; ++k) up = fmaxf(up, ml[k].x);
         const float f = s.m == kNone ? 0.f : exp2_approx(s.m - up);
         s.l *= f;
         s.o = make_float4(s.o.x * f, s.o.y * f, s.o.z * f, s.o.w * f);
 #pragma unroll
         for (int k = 0; k < kFlight; ++k) {
-            const float w = pm[k] == kNone ? 0.f : exp2_approx(pm[k] - up);
-            s.l = fmaf(w, pl[k], s.l);
+            const float w = ml[k].x == kNone ? 0.f : exp2_approx(ml[k].x - up);
+            s.l = fmaf(w, ml[k].y, s.l);
             s.o = make_float4(fmaf(w, po[k].x, s.o.x), fmaf(w, po[k].y, s.o.y), fmaf(w, po[k].z, s.o.z), fmaf(w, po[k].w, s.o.w));
         }
         s.m = up;
@@ -471,19 +480,20 @@ __device__ __forceinline__ void nothing_to_join() {
 }
 
 /* The items the split kernel cut. The pieces of an item lie in the slots of the CTAs that own its first to last block:
- * slot 1 of the first, slot 0 of the others. A CTA joins D / p.parts elements of one query head of a sequence: groups of
+ * slot 1 of the first, slot 0 of the others. A CTA joins D / kParts elements of one query head of a sequence: groups of
  * threads, four elements a thread, take every so-many-th piece with a running maximum of their own, and meet at the end. */
-template <int NT, int kFlight, int kJoinThreads>
+template <int NT, int kFlight, int kJoinThreads, int kParts>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Plan p) {
     __shared__ float4 sums[kJoinThreads];
     __shared__ float2 stats[kJoinThreads];
     const RidgeFillAttnDecode& g = p.g;
     const int tid = threadIdx.x, lane = tid & 31;
     const int n_head = (int)g.n_head, B = (int)g.B;
-    const int part = blockIdx.x % p.parts, bh = blockIdx.x / p.parts;
+    const int part = blockIdx.x % kParts, bh = blockIdx.x / kParts;
     const int b = bh / n_head, h = bh - b * n_head, in_group = h % p.group;
     const int items = (int)g.n_head_kv * p.chunks, it = h / p.group * p.chunks + in_group / (8 * NT), row = in_group % (8 * NT);
-    const int lanes = D / 4 / p.parts, groups = kJoinThreads / lanes, group = tid / lanes, d = (part * lanes + tid % lanes) * 4;
+    constexpr int lanes = D / 4 / kParts, groups = kJoinThreads / lanes;
+    const int group = tid / lanes, d = (part * lanes + tid % lanes) * 4;
     uint16_t* out = g.o + b * g.o_row + (int64_t)h * g.o_head + d;
     const int units = units_of(g, b);
     if (units == 0) {   /* no key: zeros */
@@ -509,8 +519,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Plan p) {
     __syncthreads();
     if (group > 0) return;
     float top = kNone, sum = 0.f;
+#pragma unroll
     for (int k = 0; k < groups; ++k) top = fmaxf(top, stats[tid + k * lanes].x);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
     for (int k = 0; k < groups; ++k) {
         const float2 s = stats[tid + k * lanes];
         const float4 v = sums[tid + k * lanes];
@@ -556,12 +568,12 @@ int launch(const Plan& p, bool split, cudaStream_t s) {
     if (rc != RAD_OK) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.g.B * p.g.n_head * p.parts));
-    /* Loads in flight a thread and threads a CTA, by how many pieces an item may have and how many CTAs there are. What a
-     * whole call took beside the split as it was then (it takes 2 to 60 us less now, the join the same): one sequence of
-     * 32,768 keys 24.4 us with 16 loads, 26.0 with 8; of 500: 8.0 with 2, 8.9 with 16. 32 short sequences, a few pieces each:
-     * 25.1 us with CTAs so small that all run at once, 30.3 with the registers of 16 loads. 64 long ones, a dozen pieces each:
-     * 399 us with 8 loads, 404 with the small CTAs. */
-    const bool few = p.parts > 1, many_pieces = p.g.n_pages * p.g.page > 32 * kRound;
+    /* Loads in flight a thread, threads and CTAs a head, by how many pieces an item may have and how many heads
+     * there are. One sequence of 32,768 keys, 148 pieces: 19.0 us with eight CTAs a head and 8 loads, 19.5 with four and 16; of
+     * 500 keys, five pieces: 6.3 us with four CTAs and 2 loads, 6.8 with eight and 8. 32 short sequences, a few pieces each:
+     * 20.7 us with one CTA a head, small enough that all run at once, and 5 loads; 21.5 with 4, 22.0 with 8, 21.9 with four
+     * CTAs. 64 long ones, a dozen pieces each, 8 loads: 1 % less than with the small CTAs. */
+    const bool few = p.parts > 1;
     cfg.blockDim = dim3(few || p.narrow ? 256 : 128);
     cfg.stream = s;
     cudaLaunchAttribute at;
@@ -569,8 +581,8 @@ int launch(const Plan& p, bool split, cudaStream_t s) {
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, few ? (many_pieces ? join_kernel<NT, 16, 256> : join_kernel<NT, 2, 256>)
-                                     : p.narrow ? join_kernel<NT, 8, 256> : join_kernel<NT, 4, 128>, p) != cudaSuccess) {
+    if (cudaLaunchKernelEx(&cfg, few ? (p.parts == 8 ? join_kernel<NT, 8, 256, 8> : join_kernel<NT, 2, 256, 4>)
+                                     : p.narrow ? join_kernel<NT, 8, 256, 1> : join_kernel<NT, 5, 128, 1>, p) != cudaSuccess) {
         cudaGetLastError();
         return RAD_E_DEVICE;
     }
@@ -599,8 +611,11 @@ extern "C" int ridgefill_attn_decode_device(const RadArgs* a, RadStream s) {
     p.ctas = sh.ctas;
     p.seats = sh.seats;
     p.narrow = sh.narrow;
-    /* few heads may have many pieces each: four CTAs a head share them (one sequence of 32,768: 27 us against 29 with one, when the split took 6 us more) */
-    p.parts = p.g.B * p.g.n_head <= sh.seats ? 4 : 1;
+    p.page_shift = -1;
+    for (int i = 0; i <= 20; ++i)
+        if (p.g.page == 1 << i) p.page_shift = i;
+    /* few heads may have many pieces each, which several CTAs a head share */
+    p.parts = p.g.B * p.g.n_head > sh.seats ? 1 : p.g.n_pages * p.g.page > 32 * kRound ? 8 : 4;
     p.partials = sh.split ? a->scratch : nullptr;
     p.scale_log2 = p.g.scale * 1.4426950408889634f;
     return sh.nt == 1 ? launch<1>(p, sh.split, rf::as_stream(s)) : launch<2>(p, sh.split, rf::as_stream(s));

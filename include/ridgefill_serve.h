@@ -12,6 +12,7 @@
  * a graph. Values in device memory (lengths, page and slot numbers) are read where the kernel runs, with a fail-safe:
  * cu_seqlens and lengths are clamped into their operands, a page or slot outside its pool is not read or written.
  * A call's workspace is its own until the call has run: calls that may overlap on the GPU need one each.
+ * An operand with an extent of 0 still carries an address: one without it counts as not given.
  */
 #ifndef RIDGEFILL_SERVE_H
 #define RIDGEFILL_SERVE_H

@@ -290,9 +290,22 @@ struct Order {
     }
 };
 
-/* Announces them in the ring; `owner`: the first one's, found before the barriers stood. */
-__device__ void announce(Order& order, Shared& s, int owner) {
-    for (int k = 0;; owner = order.find(++k)) {
+/* Zeros for a query tile none of whose rows has a key: this CTA's rows of it, a row's 512 bytes an instruction. */
+__device__ void clear(const Plan& p, const Shared& s, int q0, int rows, int head, int lane) {
+    uint16_t* const out = p.g.o + (int64_t)q0 * p.g.o_row + (int64_t)(head * p.group) * p.g.o_head;
+    for (int r = 0; r < rows * p.group; ++r) *(uint4*)(out + s.at[r] + 8 * lane) = make_uint4(0u, 0u, 0u, 0u);
+}
+
+/* Announces them in the ring; `owner`: the first one's, found before the barriers stood. A query tile without keys never
+ * enters it: the products' warp looks one tile ahead, and a row of such tiles would fill the ring before the output's warps
+ * have done the last one with keys, each waiting for the other. */
+__device__ void announce(const Plan& p, Order& order, Shared& s, int owner) {
+    for (int k = 0, n = 0;; owner = order.find(++n)) {
+        if (owner >= 0 && __shfl_sync(0xffffffffu, order.own.tiles, owner) == 0) {
+            clear(p, s, __shfl_sync(0xffffffffu, order.own.q0, owner), __shfl_sync(0xffffffffu, order.own.rows, owner),
+                  __shfl_sync(0xffffffffu, order.own.head, owner), order.lane);
+            continue;
+        }
         const int slot = k % kRing;
         if (!rf::mbar_wait(&s.item_empty[slot], ((k / kRing) & 1) ^ 1, &s.abort, rf::kErrAttnWait)) return;
         __syncwarp();
@@ -302,6 +315,7 @@ __device__ void announce(Order& order, Shared& s, int owner) {
             rf::mbar_arrive(&s.item_full[slot]);
         }
         if (owner < 0) return;
+        ++k;
     }
 }
 
@@ -335,7 +349,6 @@ __device__ void produce(const Plan& p, Shared& s, uint8_t* qtile, uint8_t* ring,
     for (;;) {
         const Item it = items.next(lane);
         if (it.rows < 0) break;
-        if (it.tiles == 0) continue;
         if (lane == 0 && ok) {
             /* a stage: 64 rows of two 64-element columns from element x */
             auto stage = [&](const CUtensorMap* map, int x, int row) {
@@ -401,15 +414,13 @@ __device__ void multiply(Shared& s, const uint8_t* qtile, const uint8_t* ring, u
     Item it = {}, ahead = {};   /* the query tiles of the PV and of the scores under way */
     int j = -1, ja = 0;         /* their key tiles; j -1: no PV yet */
     for (bool first = true; ok;) {
-        /* the scores' key tile: the next of this query tile, or the first of the next with keys */
+        /* the scores' key tile: the next of this query tile, or the first of the next */
         if (first) {
-            do {
-                const Item i = items.next(lane);
-                ahead.rows = __shfl_sync(0xffffffffu, i.rows, 0);
-                ahead.tiles = __shfl_sync(0xffffffffu, i.tiles, 0);
-                ahead.keys = __shfl_sync(0xffffffffu, i.keys, 0);
-                ahead.first = __shfl_sync(0xffffffffu, i.first, 0);
-            } while (ahead.rows >= 0 && ahead.tiles == 0);
+            const Item i = items.next(lane);
+            ahead.rows = __shfl_sync(0xffffffffu, i.rows, 0);
+            ahead.tiles = __shfl_sync(0xffffffffu, i.tiles, 0);
+            ahead.keys = __shfl_sync(0xffffffffu, i.keys, 0);
+            ahead.first = __shfl_sync(0xffffffffu, i.first, 0);
             ja = 0;
         }
         const bool more = ahead.rows >= 0;
@@ -485,7 +496,6 @@ __device__ void soften(const Plan& p, Shared& s, uint32_t tmem, int warp, int la
         /* the two warps of these rows meet once a query tile and once a key tile, and leave together: when a wait gave up
          * neither is left at a barrier */
         if (rf::bar_any(1 + quarter, 64, it.rows < 0)) return;
-        if (it.tiles == 0) continue;
         const int limit = it.limit + min(token, max(it.rows - 1, 0));   /* this row's last key */
         float m = kNone, l0 = 0.f, l1 = 0.f;
         buf = buf == 2 ? 0 : buf + 1;
@@ -582,10 +592,6 @@ __device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, u
         if (it.rows < 0) return;
         const int live = it.rows * p.group;   /* this CTA's rows */
         uint16_t* const out = g.o + (int64_t)it.q0 * g.o_row + (int64_t)(it.head * p.group) * g.o_head;
-        if (it.tiles == 0) {   /* no row of the tile has a key */
-            for (int r = warp * 32; r < min(warp * 32 + 32, live); ++r) *(uint4*)(out + s.at[r] + 8 * lane) = make_uint4(0u, 0u, 0u, 0u);
-            continue;
-        }
         use += 4 * it.tiles;
         if ((it.first + it.tiles) * kTileN > it.keys) {   /* V rows of the last tile past the sequence: the last two stages, 64 rows each */
             const bool ok = rf::mbar_wait(&s.v_last, partial++ & 1, &s.abort, rf::kErrAttnWait);
@@ -717,7 +723,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         Order order(p, rank, lane);
         const int owner = order.find(0);
         rf::cluster_sync_all();
-        announce(order, s, owner);
+        announce(p, order, s, owner);
         rf::cluster_sync_all();
         return;
     }

@@ -79,6 +79,18 @@ def test_rows_without_keys(cuda, product_lib, nq, nk):
     assert (d["o"][:nq - nk] == 0).all()
 
 
+@pytest.mark.parametrize("nq,nk,hq,hkv", [([1033, 1033], [443, 1033], 96, 3), ([6000], [50], 8, 1), ([3000, 100], [0, 100], 128, 1),
+                                          ([200] * 40, [0, 200] * 20, 64, 2), ([900, 64] * 20, [1, 64] * 20, 32, 1)])
+def test_many_query_tiles_without_keys(cuda, product_lib, nq, nk, hq, hkv):
+    """Whole rows of query tiles that no key reaches, behind tiles with keys and between them: zeros, and the rest unharmed."""
+    torch = cuda
+    d = inputs(torch, 65, nq, nk, hq, hkv)
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, d, heads=[0, hq // 2, hq - 1])
+    for q0, n, k in zip(d["cu_q"], nq, nk):
+        assert (d["o"][q0:q0 + max(n - k, 0)] == 0).all()
+
+
 @pytest.mark.parametrize("hq,hkv", [(1, 1), (2, 2), (4, 1), (12, 2), (9, 3), (16, 1), (20, 1), (48, 3), (100, 1), (128, 1), (130, 2)])
 def test_head_groups(cuda, product_lib, hq, hkv):
     torch = cuda

@@ -266,3 +266,26 @@ def test_next_kernel_sees_the_answer(cuda, product_lib, lens):
             d["o"].fill_(7.0)
             stream.synchronize()
             check(torch, dict(d, o=seen))
+
+
+def test_a_replay_takes_the_lengths_of_its_moment(cuda, product_lib):
+    """One captured call, replayed while the sequences grow, shrink to nothing and change places in the table."""
+    torch = cuda
+    top = [30000, 5000, 700, 64, 1, 0]
+    d = inputs(torch, 53, top, 16, 2, 64)
+    ops, params = [H.dev(d[n]) for n in ("q", "cache", "table", "lens", "o")], S.decode_params(len(top), 16, 2, 64)
+    row = product_lib.find_row("ridgefill_attn_decode", abi.DOMAIN_DEVICE)
+    n = product_lib.scratch_bytes(row, ops, params)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    bound = product_lib.bind(row, ops, params, scratch=ws.data_ptr(), scratch_bytes=n)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert bound(torch.cuda.current_stream().cuda_stream) == abi.OK
+    for i, lens in enumerate(([30000, 5000, 700, 64, 1, 0], [1, 2, 3, 4, 1, 0], [0] * 6, [29999, 0, 700, 0, 1, 0], [17, 4999, 0, 63, 0, 0])):
+        order = torch.randperm(len(top), device="cuda")
+        d["table"].copy_(d["table"][order].clone())
+        top = [top[k] for k in order.tolist()]
+        d["lens"].copy_(torch.tensor([min(a, b) for a, b in zip(lens, top)], dtype=torch.int32))
+        d["o"].fill_(7.0)
+        graph.replay()
+        check(torch, d)

@@ -321,3 +321,28 @@ def test_lists_that_overlap(cuda, product_lib):
     o, bound, _ = S.prefill_reference(torch, d["q"], d["k"], d["v"], [0, 200], [0, 9000])
     assert ((d["o"][:100].double() - o[:100]).abs() <= bound[:100]).all()
     assert product_lib.lib.ridgefill_device_error(1) == 0
+
+
+@pytest.mark.parametrize("keys", [700, 9000])
+def test_a_replay_takes_the_lengths_of_its_moment(cuda, product_lib, keys):
+    """One captured call, whole and split, replayed with other sequences in the same rows."""
+    torch = cuda
+    d = inputs(torch, 66, [600], [keys], 16, 2)
+    cu = [torch.zeros(4, dtype=torch.int32, device="cuda") for _ in range(2)]
+    ops, params = [H.dev(d["q"]), H.dev(d["k"]), H.dev(d["v"]), H.dev(cu[0]), H.dev(cu[1]), H.dev(d["o"])], S.prefill_params(600, 16, 2)
+    row = product_lib.find_row("ridgefill_attn_prefill", abi.DOMAIN_DEVICE)
+    n = product_lib.scratch_bytes(row, ops, params)
+    ws = torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")
+    bound = product_lib.bind(row, ops, params, scratch=ws.data_ptr(), scratch_bytes=n)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert bound(torch.cuda.current_stream().cuda_stream) == abi.OK
+    for q, k in (([0, 600, 600, 600], [0, keys, keys, keys]), ([0, 1, 400, 600], [0, 1, 500, keys]), ([0] * 4, [0] * 4),
+                 ([7, 7, 300, 301], [0, 5, 290, keys]), ([0, 600, 600, 600], [0, 3, 3, 3])):
+        d["cu_q"], d["cu_k"] = q, k
+        for t, x in zip(cu, (q, k)):
+            t.copy_(torch.tensor(x, dtype=torch.int32))
+        d["o"].fill_(7.0)
+        graph.replay()
+        check(torch, d)
+    assert product_lib.lib.ridgefill_device_error(1) == 0

@@ -23,10 +23,10 @@
  *   operand pairs the keys 2c, 2c+1, 2c+8, 2c+9 of elements 64 j + 8 r .. + 7 by byte permutes, and the accumulators
  *   come out as eight consecutive elements a lane and head.
  *
- * Measured, 16 query heads over 2 kv heads, replayed from a graph: 64 sequences of 1 to 32,768 keys 335 us (6.64 TB/s, the
+ * Measured, 16 query heads over 2 kv heads, replayed from a graph: 64 sequences of 1 to 32,768 keys 334 us (6.66 TB/s, the
  * measured copy rate), one of 32,768 keys 19.0 us (67 MB: 10.3 us at that rate; the rest is the lengths' and the tables' way
  * from memory, 2.5 us, the first and last rows' ramp, 2, the warps' meeting, 1, and the join, 3), 32 of 256 to 2,038 keys
- * 20.7 us (77 MB), one of 500 keys 6.3 us.
+ * 20.7 us (77 MB), one of 500 keys 6.4 us.
  */
 #include <cuda_bf16.h>
 
@@ -337,7 +337,7 @@ __device__ __forceinline__ void run_piece(const Plan& p, uint8_t* smem, int b, i
 /* The units cut into spans, CTA i taking span i. `seats` CTAs run at a time.
  * With few units: as many CTAs as have one for each of their warps, at most one a seat, equal spans.
  * From kLong units a seat on: SMs do not get equal shares of the memory's rate, so equal spans leave some idle at the
- * end (64 sequences of up to 32,768: 412 us against 456 when this was chosen, 338 now). One wide span a seat takes 4/5 of the units, and four
+ * end (64 sequences of up to 32,768: 412 us against 456 when this was chosen, 334 now). One wide span a seat takes 4/5 of the units, and four
  * times as many narrow ones follow, which the hardware gives to whichever seat comes free. */
 constexpr int kLong = 128, kNarrowPerSeat = 4;
 struct Spans {

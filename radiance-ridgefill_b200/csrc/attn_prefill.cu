@@ -28,9 +28,9 @@
  * P as bf16 costs half a bf16 step a weight, of the order of the output's own rounding; f32 elsewhere.
  *
  * Measured, 16 query heads over 2: 16,384 rows 1,364 us (1.61 PFLOP/s; the tensor pipe is active 89 % of the SMs' time),
- * 2,048 rows over 32,768 keys 672 us (1.58 PFLOP/s), 2,048 rows 33.0 us (1.04), six prompts of 256 to 2,048 rows 74 us
- * (1.10), 37 rows 10 us, each replayed from a graph for milliseconds. Run on for seconds the card is at its power limit,
- * 1,410 MHz under the long calls: 1,587, 786, 38.9 and 89 us. What the shorter ones lose lies between query tiles: the
+ * 2,048 rows over 32,768 keys 670 us (1.59 PFLOP/s), 2,048 rows 33.4 us (1.03), six prompts of 256 to 2,048 rows 74.5 us
+ * (1.09), 37 rows 10 us, each replayed from a graph for milliseconds. Run on for seconds the card is at its power limit,
+ * 1,410 MHz under the long calls: 1,582, 788, 38.8 and 88 us. What the shorter ones lose lies between query tiles: the
  * next one's PV(0) waits for O to be read: 5,100 cycles from one PV to the next there, 2,800 elsewhere.
  */
 #include <cuda_bf16.h>

@@ -162,9 +162,9 @@ __device__ __forceinline__ int lane_holding(int x, int at, int lane, int* before
  * span that holds all key tiles of a query tile writes its output; the at most two that it cuts leave Partials (slot 1 of
  * the pair that has the first of them, slot 0 of the others), which join_kernel adds up. */
 struct Spans {
-    int n, each, extra;   /* the first `extra` spans one longer; with few tiles fewer spans, of four at least */
+    int n, each, extra;   /* the first `extra` spans one longer; with few tiles fewer spans, of two at least */
     __device__ __forceinline__ Spans(int total, int most) {
-        n = max(min((total + 3) / 4, most), 1);
+        n = max(min((total + 1) / 2, most), 1);
         each = total / n;
         extra = total - each * n;
     }
@@ -614,14 +614,15 @@ __device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, u
         const float sum = s.sum[done % 3][0][row] + s.sum[done % 3][1][row];
         if (it.slot >= 0) {   /* a piece: a thread its row's sums, a column's 128 rows side by side */
             Partial& part = ((Partial*)p.partials)[((int64_t)rf::cluster_id_x() * 2 + it.slot) * 2 + rank];
-            part.ml[row] = make_float2(s.top_of[done % 3][row], sum);
+            if (row < live) part.ml[row] = make_float2(s.top_of[done % 3][row], sum);
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
                 uint32_t o[32];
                 rf::tmem_ld32(mine + 32 * c, o);
                 rf::tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) part.o[32 * c + e][row] = __uint_as_float(o[e]);
+                for (int e = 0; e < 32; ++e)
+                    if (row < live) part.o[32 * c + e][row] = __uint_as_float(o[e]);
             }
             rf::tc_fence_before();
             __syncwarp();
@@ -747,14 +748,14 @@ __device__ __forceinline__ void nothing_to_join() {
     if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-constexpr int kJoinCols = 64, kJoinParts = D / kJoinCols;
-
-/* The query tiles that the split cut, and those without a key (zeros): a CTA joins kJoinCols columns of a CTA's share of
- * one query tile and kv head, a thread a row. */
+/* The query tiles that the split cut, and those without a key (zeros): a CTA joins kCols columns of a CTA's share of one
+ * query tile and kv head, a thread a row, kFlight pieces' loads in flight. */
+template <int kCols, int kFlight>
 __global__ void __launch_bounds__(kTileM) join_kernel(const Plan p) {
     const RidgeFillAttnPrefill& g = p.g;
     const int lane = threadIdx.x & 31, row = threadIdx.x, heads = (int)g.n_head_kv;
-    const int part = blockIdx.x % kJoinParts, rank = blockIdx.x / kJoinParts % 2, item = blockIdx.x / (2 * kJoinParts);
+    constexpr int parts = D / kCols;
+    const int part = blockIdx.x % parts, rank = blockIdx.x / parts % 2, item = blockIdx.x / (2 * parts);
     const int query = item / heads, head = item - query * heads;
     int seen = 0, units = 0, start = 0, tiles = -1;
     Item it = {};
@@ -771,42 +772,64 @@ __global__ void __launch_bounds__(kTileM) join_kernel(const Plan p) {
     });
     if (tiles < 0) return nothing_to_join();   /* fewer query tiles than the grid has places for */
     const int token = row / p.group;
-    uint16_t* out = g.o + (int64_t)(it.q0 + token) * g.o_row + (int64_t)(head * p.group + row - token * p.group) * g.o_head + part * kJoinCols;
+    uint16_t* out = g.o + (int64_t)(it.q0 + token) * g.o_row + (int64_t)(head * p.group + row - token * p.group) * g.o_head + part * kCols;
     const bool live = token < it.rows;
     if (tiles == 0) {
         if (live)
-            for (int c = 0; c < kJoinCols / 8; ++c) *(uint4*)(out + 8 * c) = make_uint4(0u, 0u, 0u, 0u);
+            for (int c = 0; c < kCols / 8; ++c) *(uint4*)(out + 8 * c) = make_uint4(0u, 0u, 0u, 0u);
         return nothing_to_join();
     }
     const Spans spans(units * heads, p.pairs);
     const int c0 = spans.owner(start), n = spans.owner(start + tiles - 1) - c0 + 1;
     if (n == 1) return nothing_to_join();   /* written by its one pair */
     asm volatile("griddepcontrol.wait;" ::: "memory");   /* the split is done and its results are visible */
-    auto piece = [&](int i) -> const Partial& { return ((const Partial*)p.partials)[((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * 2 + rank]; };
-    float top = kNone, sum = 0.f, acc[kJoinCols];
-    for (int i = 0; i < n; ++i) top = fmaxf(top, piece(i).ml[row].x);
-#pragma unroll
-    for (int c = 0; c < kJoinCols; ++c) acc[c] = 0.f;
-    for (int i = 0; i < n; ++i) {
-        const Partial& s = piece(i);
-        const float2 ml = s.ml[row];
-        const float f = ml.x == kNone ? 0.f : exp2_approx(ml.x - top);
-        sum = fmaf(f, ml.y, sum);
-#pragma unroll
-        for (int c = 0; c < kJoinCols; ++c) acc[c] = fmaf(f, s.o[part * kJoinCols + c][row], acc[c]);
-    }
     if (!live) return;
+    auto piece = [&](int i) -> const Partial& { return ((const Partial*)p.partials)[((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * 2 + rank]; };
+    float top = kNone, sum = 0.f, acc[kCols];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) acc[c] = 0.f;
+    for (int i = 0; i < n; i += kFlight) {
+        float2 ml[kFlight];
+        float o[kFlight][kCols];
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) {
+            const Partial& s = piece(min(i + k, n - 1));
+            ml[k] = i + k < n ? s.ml[row] : make_float2(kNone, 0.f);
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) o[k][c] = s.o[part * kCols + c][row];
+        }
+        float up = top;
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) up = fmaxf(up, ml[k].x);
+        const float f = top == kNone ? 0.f : exp2_approx(top - up);
+        sum *= f;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) acc[c] *= f;
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) {
+            if (ml[k].x == kNone) continue;   /* no piece, or none of its keys is the row's */
+            const float w = exp2_approx(ml[k].x - up);
+            sum = fmaf(w, ml[k].y, sum);
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) acc[c] = fmaf(w, o[k][c], acc[c]);
+        }
+        top = up;
+    }
     const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
 #pragma unroll
-    for (int c = 0; c < kJoinCols; c += 8)
+    for (int c = 0; c < kCols; c += 8)
         *(uint4*)(out + c) = make_uint4(pack(acc[c] * inv, acc[c + 1] * inv), pack(acc[c + 2] * inv, acc[c + 3] * inv),
                                         pack(acc[c + 4] * inv, acc[c + 5] * inv), pack(acc[c + 6] * inv, acc[c + 7] * inv));
 }
 
-/* How a parsed call runs. Query tiles go to pairs whole where there are many; with two a pair or fewer and long keys (the
- * tail of a long prompt) that would leave pairs idle -- 128 query tiles of 256 key tiles on 74 pairs take two rounds, 86 % of
- * the pairs' time -- so the key tiles are split evenly instead, and the cut query tiles joined. */
-constexpr int kLongKeys = 8192;
+/* How a parsed call runs: query tiles go to pairs whole, or their key tiles are split evenly and the cut ones joined. Whole,
+ * the pair with the longest query tile decides, or the one with two. The split is taken
+ *   with fewer query tiles than pairs, when evening them out saves the longest one (a sequence's average, the lengths being
+ *   device memory) kLeast key tiles, 1.4 us each: 16 rows over 4,096 keys 20.5 us, 49 whole; 300 over 6,000 39, 69 whole; near
+ *   kLeast 64 over 1,024 17.1, 19.6 whole, and 512 over 1,500 27.5, 26 whole
+ *   with at most two a pair and keys from kLongKeys on: 2,048 rows over 32,768, 128 query tiles of 256 key tiles on 74 pairs,
+ *   would take two rounds, 86 % of the pairs' time: 670 us, 704 whole */
+constexpr int kLongKeys = 8192, kLeast = 6;
 struct Shape {
     int group, tokens;
     int64_t items;      /* query tiles (of all kv heads) at most: a sequence's last one may be cut short */
@@ -820,8 +843,10 @@ Shape shape_of(const RidgeFillAttnPrefill& g) {
     s.tokens = kTileM / s.group;
     s.items = (g.T / (2 * s.tokens) + g.n_seq) * g.n_head_kv;
     s.pairs = rf::sm_count() / 2;
+    const bool few = s.items < s.pairs && g.Tk * (s.pairs - s.items) >= (int64_t)kLeast * kTileN * s.pairs * g.n_seq;
+    const bool two = s.items <= 2 * s.pairs && g.Tk >= kLongKeys;
     /* the split counts key tiles in 32 bits, whatever cu_seqlens and cu_keys hold: sequences that overlap too */
-    s.split = g.Tk >= kLongKeys && s.items <= 2 * s.pairs && g.n_seq * s.items * (g.Tk / kTileN + 1) <= 0x7fffffffLL;
+    s.split = (few || two) && g.n_seq * s.items * (g.Tk / kTileN + 1) <= 0x7fffffffLL;
     s.bytes = s.split ? (int64_t)s.pairs * 4 * (int64_t)sizeof(Partial) : 0;
     return s;
 }
@@ -882,7 +907,11 @@ extern "C" int ridgefill_attn_prefill_device(const RadArgs* a, RadStream s) {
     prefill_kernel<<<2 * (unsigned)pairs, kThreads, kSmemBytes, rf::as_stream(s)>>>(mq, mk, mv, p);
     if (const int launched = rf::launch_status(); launched != RAD_OK || !sh.split) return launched;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(sh.items * 2 * kJoinParts));
+    /* The join's columns a CTA and pieces in flight, by how many pieces a query tile may have. 16 rows over 32,768 keys: 44 us
+     * with 8 columns and 8 pieces, 61 with 16 and 4, 100 with 64 and one; 700 rows of 8 heads over 9,000: 67, 50 and 78; 2,048
+     * rows over 32,768, two or three pieces each: 690 with 8 columns, 680 with 64. */
+    const int cols = 3 * sh.items <= sh.pairs ? 8 : sh.items <= sh.pairs ? 16 : 64;
+    cfg.gridDim = dim3((unsigned)(sh.items * 2 * (D / cols)));
     cfg.blockDim = dim3(kTileM);
     cfg.stream = rf::as_stream(s);
     cudaLaunchAttribute at;
@@ -890,7 +919,7 @@ extern "C" int ridgefill_attn_prefill_device(const RadArgs* a, RadStream s) {
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, join_kernel, p) != cudaSuccess) {
+    if (cudaLaunchKernelEx(&cfg, cols == 8 ? join_kernel<8, 8> : cols == 16 ? join_kernel<16, 4> : join_kernel<64, 1>, p) != cudaSuccess) {
         cudaGetLastError();
         return RAD_E_DEVICE;
     }

@@ -124,6 +124,19 @@ def test_split_over_long_keys(cuda, product_lib, nq, nk):
     check(torch, d, heads=None if sum(nq) < 500 else [0, 5, 8, 15])
 
 
+@pytest.mark.parametrize("nq,nk,hq,hkv", [([16], [4096], 16, 2), ([1], [1024], 16, 2), ([300], [6000], 16, 2), ([1500], [1500], 2, 2),
+                                          ([16, 1, 1, 100], [4000, 20, 90, 300], 16, 2), ([20, 20, 400], [800, 2000, 400], 8, 1),
+                                          ([4] * 8, [1000, 900, 800, 700, 1200, 1000, 50, 3000], 16, 2), ([64], [20000], 8, 8)])
+def test_split_of_few_query_tiles(cuda, product_lib, nq, nk, hq, hkv):
+    """Fewer query tiles than pairs: cut into many pieces, a few, none."""
+    torch = cuda
+    d = inputs(torch, 68, nq, nk, hq, hkv, pad=2)
+    params, (ops, keep) = S.prefill_params(d["q"].shape[0], hq, hkv), operands(torch, d)
+    assert product_lib.scratch_bytes(product_lib.find_row("ridgefill_attn_prefill", abi.DOMAIN_DEVICE), ops, params) > 0
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, d, heads=sorted({0, hq // 2, hq - 1}))
+
+
 @pytest.mark.parametrize("hq,hkv", [(3, 1), (12, 2), (40, 1), (128, 1)])
 def test_split_head_groups(cuda, product_lib, hq, hkv):
     torch = cuda
@@ -217,6 +230,24 @@ def test_nan_stays_in_its_sequence(cuda, product_lib):
     assert same[:100].all() and same[300:].all() and same[100:150].all()
     assert torch.isnan(got[150]).all() and torch.isnan(got[299]).all()
     check(torch, clean)
+
+
+@pytest.mark.parametrize("nq,nk,hq,hkv,at", [(700, 700, 16, 2, 500), (700, 700, 2, 2, 600), (300, 9000, 16, 2, 8900), (520, 6000, 3, 3, 5800),
+                                             (40, 2000, 8, 1, 1970)])
+def test_how_far_a_nan_value_reaches(cuda, product_lib, nq, nk, hq, hkv, at):
+    """A NaN in v: every row that sees it is NaN, rows whose last key lies more than 126 + 256 / group before it are as
+    without it. Whole query tiles and split ones."""
+    torch = cuda
+    d = inputs(torch, 67, [nq], [nk], hq, hkv)
+    assert call(product_lib, torch, d) == abi.OK
+    clean = d["o"].clone()
+    check(torch, d)
+    d["v"][at] = float("nan")
+    assert call(product_lib, torch, d) == abi.OK
+    first = at - (nk - nq)   # the first row that sees it
+    assert torch.isnan(d["o"][max(first, 0):]).all()
+    far = first - (126 + 256 // (hq // hkv))
+    assert far <= 0 or torch.equal(d["o"][:far], clean[:far])
 
 
 def test_more_than_32_bits_of_keys(cuda, product_lib):

@@ -825,8 +825,8 @@ __global__ void __launch_bounds__(kTileM) join_kernel(const Plan p) {
 /* How a parsed call runs: query tiles go to pairs whole, or their key tiles are split evenly and the cut ones joined. Whole,
  * the pair with the longest query tile decides, or the one with two. The split is taken
  *   with fewer query tiles than pairs, when evening them out saves the longest one (a sequence's average, the lengths being
- *   device memory) kLeast key tiles, 1.4 us each: 16 rows over 4,096 keys 20.5 us, 49 whole; 300 over 6,000 39, 69 whole; near
- *   kLeast 64 over 1,024 17.1, 19.6 whole, and 512 over 1,500 27.5, 26 whole
+ *   device memory) kLeast key tiles, 1.4 us each: 16 rows over 4,096 keys 17 us, 49 whole; 300 over 6,000 38, 69 whole; near
+ *   kLeast 64 over 1,024 15, 19.6 whole, and 512 over 1,500 27.5, 26 whole
  *   with at most two a pair and keys from kLongKeys on: 2,048 rows over 32,768, 128 query tiles of 256 key tiles on 74 pairs,
  *   would take two rounds, 86 % of the pairs' time: 670 us, 704 whole */
 constexpr int kLongKeys = 8192, kLeast = 6;
@@ -907,9 +907,9 @@ extern "C" int ridgefill_attn_prefill_device(const RadArgs* a, RadStream s) {
     prefill_kernel<<<2 * (unsigned)pairs, kThreads, kSmemBytes, rf::as_stream(s)>>>(mq, mk, mv, p);
     if (const int launched = rf::launch_status(); launched != RAD_OK || !sh.split) return launched;
     cudaLaunchConfig_t cfg = {};
-    /* The join's columns a CTA and pieces in flight, by how many pieces a query tile may have. 16 rows over 32,768 keys: 44 us
-     * with 8 columns and 8 pieces, 61 with 16 and 4, 100 with 64 and one; 700 rows of 8 heads over 9,000: 67, 50 and 78; 2,048
-     * rows over 32,768, two or three pieces each: 690 with 8 columns, 680 with 64. */
+    /* The join's columns a CTA and pieces in flight, by how many pieces a query tile may have. 16 rows over 32,768 keys: 35 us
+     * with 8 columns and 8 pieces, 46 with 16 and 4, 98 with 64 and one; 300 rows over 6,000: 39.4, 37.9 and 47.2; 1,024 rows
+     * over 16,384: 191, 184 and 185; 2,048 over 32,768, eight launches in a row: 704, 758 and 701. */
     const int cols = 3 * sh.items <= sh.pairs ? 8 : sh.items <= sh.pairs ? 16 : 64;
     cfg.gridDim = dim3((unsigned)(sh.items * 2 * (D / cols)));
     cfg.blockDim = dim3(kTileM);

@@ -136,10 +136,12 @@ extern "C" int ridgefill_gdn_step_device(const RadArgs* a, RadStream s) {
     if (rc != RAD_OK) return rc;
     if (g.B == 0) return RAD_OK;
     cudaStream_t stream = rf::as_stream(s);
-    if (g.dk <= 32) return launch<1, 1>(g, stream);
-    if (g.dk <= 64) return launch<2, 1>(g, stream);
-    /* 64-row CTAs stream best (four rows a lane in flight; 161 us at 256 rows of 32 heads, 208 with 16-row ones); while a head
-     * an SM would leave SMs idle, 16-row ones spread a head over eight */
-    if (g.B * g.n_head_v <= rf::sm_count()) return launch<4, 1>(g, stream);
+    /* Several state rows a lane in flight stream best (256 rows of 32 heads: of 128, 161 us with 64-row CTAs, 208 with 16-row
+     * ones; of 64, 48 us with 32-row ones, 77 with 16; of 32, 24 and 38); while a head an SM would leave SMs idle, 16-row CTAs
+     * spread a head over more of them */
+    const bool spread = g.B * g.n_head_v <= rf::sm_count();
+    if (g.dk <= 32) return spread ? launch<1, 1>(g, stream) : launch<1, 2>(g, stream);
+    if (g.dk <= 64) return spread ? launch<2, 1>(g, stream) : launch<2, 2>(g, stream);
+    if (spread) return launch<4, 1>(g, stream);
     return launch<4, 4>(g, stream);
 }

@@ -64,6 +64,16 @@ def test_small_heads(cuda, product_lib, dk, dv):
     check(torch, d, before, scale=0.7)
 
 
+@pytest.mark.parametrize("dk,dv", [(8, 1), (32, 33), (24, 64), (64, 63), (40, 31)])
+def test_small_heads_of_a_large_batch(cuda, product_lib, dk, dv):
+    """More heads than SMs: the form with several state rows a lane, cut anywhere."""
+    torch = cuda
+    d = inputs(torch, dk + dv, 70, 2, 6, dk, dv)
+    before = d["state"].clone()
+    assert call(product_lib, d) == abi.OK
+    check(torch, d, before)
+
+
 def test_strided_operands(cuda, product_lib):
     """q, k, v as slices of one projected row, g and beta with a row pitch, slot pitch and head pitch of the pool
     above the packed ones, o into a wider row, slot numbers in a [B, 2] table's first column."""

@@ -23,10 +23,10 @@
  *   operand pairs the keys 2c, 2c+1, 2c+8, 2c+9 of elements 64 j + 8 r .. + 7 by byte permutes, and the accumulators
  *   come out as eight consecutive elements a lane and head.
  *
- * Measured, 16 query heads over 2 kv heads, replayed from a graph: 64 sequences of 1 to 32,768 keys 334 us (6.66 TB/s, the
+ * Measured, 16 query heads over 2 kv heads, replayed from a graph: 64 sequences of 1 to 32,768 keys 332 us (6.71 TB/s, the
  * measured copy rate), one of 32,768 keys 19.0 us (67 MB: 10.3 us at that rate; the rest is the lengths' and the tables' way
  * from memory, 2.5 us, the first and last rows' ramp, 2, the warps' meeting, 1, and the join, 3), 32 of 256 to 2,038 keys
- * 20.7 us (77 MB), one of 500 keys 6.4 us.
+ * 20.8 us (77 MB), one of 500 keys 6.4 us.
  */
 #include <cuda_bf16.h>
 
@@ -337,15 +337,17 @@ __device__ __forceinline__ void run_piece(const Plan& p, uint8_t* smem, int b, i
 /* The units cut into spans, CTA i taking span i. `seats` CTAs run at a time.
  * With few units: as many CTAs as have one for each of their warps, at most one a seat, equal spans.
  * From kLong units a seat on: SMs do not get equal shares of the memory's rate, so equal spans leave some idle at the
- * end (64 sequences of up to 32,768: 412 us against 456 when this was chosen, 334 now). One wide span a seat takes 4/5 of the units, and four
- * times as many narrow ones follow, which the hardware gives to whichever seat comes free. */
-constexpr int kLong = 128, kNarrowPerSeat = 4;
+ * end. One wide span a seat takes 7/8 of the units, and twice as many narrow ones follow, which the hardware gives to
+ * whichever seat comes free: 332 us for 64 sequences of up to 32,768 keys, 347 with equal spans, 334 with 4/5 and four times
+ * as many. A table wide enough for that over short sequences costs the narrow spans' CTAs, which find no work: 25 us for
+ * 64 sequences of some 500 keys, 21.5 without them. */
+constexpr int kLong = 128, kNarrowPerSeat = 2;
 struct Spans {
     int n_wide = 0, wide = 0, n = 0, each = 0, extra = 0;   /* n equal spans after the wide ones, the first `extra` one longer */
     __device__ __forceinline__ Spans(int total, int seats, bool narrow) {
         if (narrow && total / kLong >= seats) {
             n_wide = seats;
-            wide = total / seats * 4 / 5;
+            wide = total / seats * 7 / 8;
             n = kNarrowPerSeat * seats;
         } else {
             n = min((total + kWarps - 1) / kWarps, seats);
@@ -568,13 +570,15 @@ int launch(const Plan& p, bool split, cudaStream_t s) {
     if (rc != RAD_OK) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.g.B * p.g.n_head * p.parts));
-    /* Loads in flight a thread, threads and CTAs a head, by how many pieces an item may have and how many heads
-     * there are. One sequence of 32,768 keys, 148 pieces: 19.0 us with eight CTAs a head and 8 loads, 19.5 with four and 16; of
-     * 500 keys, five pieces: 6.3 us with four CTAs and 2 loads, 6.8 with eight and 8. 32 short sequences, a few pieces each:
-     * 20.7 us with one CTA a head, small enough that all run at once, and 5 loads; 21.5 with 4, 22.0 with 8, 21.9 with four
-     * CTAs. 64 long ones, a dozen pieces each, 8 loads: 1 % less than with the small CTAs. */
-    const bool few = p.parts > 1;
-    cfg.blockDim = dim3(few || p.narrow ? 256 : 128);
+    /* Loads in flight a thread, threads and CTAs a head, by how many pieces an item may have and how many heads there are,
+     * all of whose CTAs should run at once: they wait on the SMs for the split's end. One sequence of 32,768 keys, 148 pieces:
+     * 19.0 us with eight CTAs a head and 8 loads, 19.5 with four and 16; of 500 keys, five pieces: 6.4 us with four CTAs and 2
+     * loads, 6.8 with eight and 8. Eight sequences of up to 32,768: 17.2 us with four CTAs and 2 loads, 23.8 with eight and 8.
+     * 32 short sequences, a few pieces each: 20.8 us with one CTA a head, small, and 5 loads; 21.5 with 4, 22.0 with 8, 21.9
+     * with four CTAs; 16 of up to 20,000: 45.6, 60 with eight CTAs. Narrow spans and fewer items than seats, a dozen pieces
+     * each: 8 loads, 1 % less than with the small CTAs for 64 long ones. */
+    const bool few = p.parts > 1, many = p.narrow && p.g.B * p.g.n_head_kv * p.chunks < p.seats;
+    cfg.blockDim = dim3(few || many ? 256 : 128);
     cfg.stream = s;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -582,7 +586,7 @@ int launch(const Plan& p, bool split, cudaStream_t s) {
     cfg.attrs = &at;
     cfg.numAttrs = 1;
     if (cudaLaunchKernelEx(&cfg, few ? (p.parts == 8 ? join_kernel<NT, 8, 256, 8> : join_kernel<NT, 2, 256, 4>)
-                                     : p.narrow ? join_kernel<NT, 8, 256, 1> : join_kernel<NT, 5, 128, 1>, p) != cudaSuccess) {
+                                     : many ? join_kernel<NT, 8, 256, 1> : join_kernel<NT, 5, 128, 1>, p) != cudaSuccess) {
         cudaGetLastError();
         return RAD_E_DEVICE;
     }
@@ -614,8 +618,9 @@ extern "C" int ridgefill_attn_decode_device(const RadArgs* a, RadStream s) {
     p.page_shift = -1;
     for (int i = 0; i <= 20; ++i)
         if (p.g.page == 1 << i) p.page_shift = i;
-    /* few heads may have many pieces each, which several CTAs a head share */
-    p.parts = p.g.B * p.g.n_head > sh.seats ? 1 : p.g.n_pages * p.g.page > 32 * kRound ? 8 : 4;
+    /* few heads may have many pieces each, which several CTAs a head share; launch() has the figures */
+    const int64_t heads = p.g.B * p.g.n_head;
+    p.parts = 8 * heads <= sh.seats && p.g.n_pages * p.g.page > 32 * kRound ? 8 : 4 * heads <= 2 * sh.seats ? 4 : 1;
     p.partials = sh.split ? a->scratch : nullptr;
     p.scale_log2 = p.g.scale * 1.4426950408889634f;
     return sh.nt == 1 ? launch<1>(p, sh.split, rf::as_stream(s)) : launch<2>(p, sh.split, rf::as_stream(s));

@@ -831,9 +831,10 @@ __global__ void __launch_bounds__(kTileM) join_kernel(const Plan p) {
 
 /* How a parsed call runs: query tiles go to pairs whole, or their key tiles are split evenly and the cut ones joined. Whole,
  * the pair with the longest query tile decides, or the one with two. The split is taken
- *   with fewer query tiles than pairs, when evening them out saves the longest one (a sequence's average, the lengths being
- *   device memory) kLeast key tiles, 1.4 us each: 16 rows over 4,096 keys 17 us, 49 whole; 300 over 6,000 38, 69 whole; near
- *   kLeast 64 over 1,024 15, 19.6 whole, and 512 over 1,500 27.5, 26 whole
+ *   with fewer query tiles than pairs, when evening them out saves the longest one kLeast key tiles, 1.4 us each (the lengths
+ *   are device memory: a sequence of about twice the average stands for the longest): 16 rows over 4,096 keys 17 us, 49
+ *   whole; 300 over 6,000 38, 69 whole; nine short tails, one of them over 6,193 keys, 26, 70 whole; near kLeast 64 over 1,024
+ *   15, 19.6 whole, and 512 over 1,500 27.5, 26 whole; eight tails over 1,000 keys each 24.5, 19.5 whole
  *   with at most two a pair and keys from kLongKeys on: 2,048 rows over 32,768, 128 query tiles of 256 key tiles on 74 pairs,
  *   would take two rounds, 86 % of the pairs' time: 670 us, 704 whole */
 constexpr int kLongKeys = 8192, kLeast = 6;
@@ -850,7 +851,7 @@ Shape shape_of(const RidgeFillAttnPrefill& g) {
     s.tokens = kTileM / s.group;
     s.items = (g.T / (2 * s.tokens) + g.n_seq) * g.n_head_kv;
     s.pairs = rf::sm_count() / 2;
-    const bool few = s.items < s.pairs && g.Tk * (s.pairs - s.items) >= (int64_t)kLeast * kTileN * s.pairs * g.n_seq;
+    const bool few = s.items < s.pairs && 2 * g.Tk * (s.pairs - s.items) >= (int64_t)kLeast * kTileN * s.pairs * (g.n_seq + 1);
     const bool two = s.items <= 2 * s.pairs && g.Tk >= kLongKeys;
     /* the split counts key tiles in 32 bits, whatever cu_seqlens and cu_keys hold: sequences that overlap too */
     s.split = (few || two) && g.n_seq * s.items * (g.Tk / kTileN + 1) <= 0x7fffffffLL;

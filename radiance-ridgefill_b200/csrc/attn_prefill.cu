@@ -835,9 +835,11 @@ __global__ void __launch_bounds__(kTileM) join_kernel(const Plan p) {
  *   are device memory: a sequence of about twice the average stands for the longest): 16 rows over 4,096 keys 17 us, 49
  *   whole; 300 over 6,000 38, 69 whole; nine short tails, one of them over 6,193 keys, 26, 70 whole; near kLeast 64 over 1,024
  *   15, 19.6 whole, and 512 over 1,500 27.5, 26 whole; eight tails over 1,000 keys each 24.5, 19.5 whole
- *   with at most two a pair and keys from kLongKeys on: 2,048 rows over 32,768, 128 query tiles of 256 key tiles on 74 pairs,
- *   would take two rounds, 86 % of the pairs' time: 670 us, 704 whole */
-constexpr int kLongKeys = 8192, kLeast = 6;
+ *   with at most two a pair, keys from kLongKeys on and a sequence of twice the average from kLongAverage: 2,048 rows over
+ *   32,768, 128 query tiles of 256 key tiles on 74 pairs, would take two rounds, 86 % of the pairs' time: 670 us, 704 whole;
+ *   four times 300 over 3,000 61, 70 whole; eight times 128 over 1,200 41, 25 whole; 30 times 2 over 300 63, 14 whole: the
+ *   split goes through the sequences one by one */
+constexpr int kLongKeys = 8192, kLongAverage = 4096, kLeast = 6;
 struct Shape {
     int group, tokens;
     int64_t items;      /* query tiles (of all kv heads) at most: a sequence's last one may be cut short */
@@ -852,7 +854,7 @@ Shape shape_of(const RidgeFillAttnPrefill& g) {
     s.items = (g.T / (2 * s.tokens) + g.n_seq) * g.n_head_kv;
     s.pairs = rf::sm_count() / 2;
     const bool few = s.items < s.pairs && 2 * g.Tk * (s.pairs - s.items) >= (int64_t)kLeast * kTileN * s.pairs * (g.n_seq + 1);
-    const bool two = s.items <= 2 * s.pairs && g.Tk >= kLongKeys;
+    const bool two = s.items <= 2 * s.pairs && g.Tk >= kLongKeys && 2 * g.Tk >= (int64_t)kLongAverage * (g.n_seq + 1);
     /* the split counts key tiles in 32 bits, whatever cu_seqlens and cu_keys hold: sequences that overlap too */
     s.split = (few || two) && g.n_seq * s.items * (g.Tk / kTileN + 1) <= 0x7fffffffLL;
     s.bytes = s.split ? (int64_t)s.pairs * 4 * (int64_t)sizeof(Partial) : 0;

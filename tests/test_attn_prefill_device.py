@@ -118,8 +118,10 @@ def test_split_over_long_keys(cuda, product_lib, nq, nk):
     d = inputs(torch, 80 + sum(nq), nq, nk, 16, 2, pad=3)
     ops, keep = operands(torch, d)
     row = product_lib.find_row("ridgefill_attn_prefill", abi.DOMAIN_DEVICE)
-    assert product_lib.scratch_bytes(row, ops, S.prefill_params(d["q"].shape[0], 16, 2)) > 0
-    assert product_lib.launch(row, ops, S.prefill_params(d["q"].shape[0], 16, 2)) == abi.E_INVAL      # without its workspace
+    split = product_lib.scratch_bytes(row, ops, S.prefill_params(d["q"].shape[0], 16, 2)) > 0
+    assert split == (len(nq) < 40)   # many sequences of some 1,000 keys are quicker whole
+    if split:
+        assert product_lib.launch(row, ops, S.prefill_params(d["q"].shape[0], 16, 2)) == abi.E_INVAL      # without its workspace
     assert call(product_lib, torch, d) == abi.OK
     check(torch, d, heads=None if sum(nq) < 500 else [0, 5, 8, 15])
 

@@ -379,3 +379,34 @@ def test_a_replay_takes_the_lengths_of_its_moment(cuda, product_lib, keys):
         graph.replay()
         check(torch, d)
     assert product_lib.lib.ridgefill_device_error(1) == 0
+
+
+@pytest.mark.parametrize("nq,nk,hq,hkv", [([40], [9000], 16, 2), ([300, 20], [6000, 400], 16, 2), ([64], [20000], 8, 8)])
+def test_nan_in_a_split_call(cuda, product_lib, nq, nk, hq, hkv):
+    """A NaN in a row of q, or in keys that fill whole pieces of it, makes the row NaN as it does in whole query tiles, where
+    the maximum of its scores passes over it; the other rows and heads are as without it."""
+    torch = cuda
+    row = product_lib.find_row("ridgefill_attn_prefill", abi.DOMAIN_DEVICE)
+
+    def clean():
+        return inputs(torch, 69, nq, nk, hq, hkv)
+
+    d = clean()
+    assert product_lib.scratch_bytes(row, operands(torch, d)[0], S.prefill_params(sum(nq), hq, hkv)) > 0
+    assert call(product_lib, torch, d) == abi.OK
+    want = d["o"]
+    d = clean()
+    d["q"][17, 3, 100] = float("nan")
+    d["q"][nq[0] - 1, 0] = float("nan")
+    assert call(product_lib, torch, d) == abi.OK
+    assert torch.isnan(d["o"][17, 3]).all() and torch.isnan(d["o"][nq[0] - 1, 0]).all()
+    d["o"][17, 3], d["o"][nq[0] - 1, 0] = want[17, 3], want[nq[0] - 1, 0]
+    assert torch.equal(d["o"], want)
+    group = hq // hkv
+    for first, last in ((0, nk[0]), (128, 4096), (2000, 2001)):   # every key of the sequence, those of whole pieces, one key
+        d = clean()
+        d["k"][first:last, 1, 77] = float("nan")
+        assert call(product_lib, torch, d) == abi.OK
+        assert torch.isnan(d["o"][:nq[0], group:2 * group]).all(), (first, last)
+        d["o"][:nq[0], group:2 * group] = want[:nq[0], group:2 * group]
+        assert torch.equal(d["o"], want)

@@ -214,10 +214,11 @@ class Plugin:
         return [self.lib.ridgefill_serve_at(i).contents for i in range(n)]
 
     def find_row(self, op: str, domain: int) -> RadKernelInfo | None:
-        if self._found is None:   # the tables are constant: read once
-            self._found = {}
+        if self._found is None:   # the tables are constant: read once, and kept when complete (other threads look too)
+            found = {}
             for r in self.rows() + self.serve_rows():
-                self._found.setdefault((r.op.decode(), r.domain), r)
+                found.setdefault((r.op.decode(), r.domain), r)
+            self._found = found
         return self._found.get((op, domain))
 
     @staticmethod

@@ -233,3 +233,30 @@ def test_decode_needs_its_workspace(product_lib):
     assert product_lib.launch(row, tensors, params) == abi.E_INVAL
     assert product_lib.launch(row, tensors, params, scratch=BASE, scratch_bytes=need - 1) == abi.E_INVAL
     assert product_lib.launch(row, tensors, params, scratch=BASE + 8, scratch_bytes=need) == abi.E_INVAL
+
+
+def test_rows_found_by_several_threads():
+    """A library's first lookups from two threads at once: the second one, while the first still reads the tables, finds its
+    row too."""
+    import threading
+    H.build_product()
+    lib = abi.Plugin(abi.PRODUCT_SO)
+    inside, go, read = threading.Event(), threading.Event(), lib.rows
+
+    def slow():
+        lib.rows = read
+        inside.set()
+        assert go.wait(30)
+        return read()
+
+    lib.rows = slow
+    got = []
+    first = threading.Thread(target=lambda: got.append(lib.find_row("ridgefill_gdn_step", abi.DOMAIN_DEVICE)))
+    first.start()
+    assert inside.wait(30)
+    second = lib.find_row("ridgefill_gdn_fill", abi.DOMAIN_DEVICE)
+    go.set()
+    first.join()
+    assert second is not None and second.op == b"ridgefill_gdn_fill"
+    assert got[0] is not None and got[0].op == b"ridgefill_gdn_step"
+    assert lib.find_row("no_such_row", abi.DOMAIN_DEVICE) is None

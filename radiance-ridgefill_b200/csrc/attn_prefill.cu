@@ -446,15 +446,19 @@ __device__ void multiply(Shared& s, const uint8_t* qtile, const uint8_t* ring, u
         if (j >= 0) {
             const bool last = j + 1 == it.tiles, cut = last && (it.first + it.tiles) * kTileN > it.keys;
             if (cut) {   /* the last V rows have landed: those past the sequence may be cleared, in both CTAs */
-                if (!wait(full(v), phase(v), full(v + 1), phase(v + 1), full(v), phase(v), full(v), phase(v))) break;
-                if (lane < 2) rf::mbar_arrive_remote(rf::map_rank(rf::smem_addr(&s.v_last), lane));
+                const uint32_t u = v + (lane & 1);   /* the copies of both CTAs complete here: acquired and released at cluster scope */
+                ok = rf::mbar_wait_lanes<true>(full(u), phase(u), &s.abort, rf::kErrAttnWait);
+                if (!ok) break;
+                if (lane < 2) rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.v_last), lane));
                 __syncwarp();
             }
             uint64_t* p = &s.p_full[tile & 1];
             const uint32_t pp = (tile >> 1) & 1;
             if (!wait(p, pp, full(v), phase(v), full(v + 1), phase(v + 1), j == 0 ? &s.o_empty : p, j == 0 ? (done & 1) ^ 1 : pp)) break;
-            if (cut && !wait(&s.v_clean, partial & 1, &s.v_clean, partial & 1, &s.v_clean, partial & 1, &s.v_clean, partial & 1)) break;
-            partial += cut;
+            if (cut) {   /* the zeros of both CTAs, before the product that reads them */
+                ok = rf::mbar_wait_lanes<true>(&s.v_clean, partial++ & 1, &s.abort, rf::kErrAttnWait);
+                if (!ok) break;
+            }
             const uint32_t a = tmem + (tile & 1) * kTileN;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -594,7 +598,7 @@ __device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, u
         uint16_t* const out = g.o + (int64_t)it.q0 * g.o_row + (int64_t)(it.head * p.group) * g.o_head;
         use += 4 * it.tiles;
         if ((it.first + it.tiles) * kTileN > it.keys) {   /* V rows of the last tile past the sequence: the last two stages, 64 rows each */
-            const bool ok = rf::mbar_wait(&s.v_last, partial++ & 1, &s.abort, rf::kErrAttnWait);
+            const bool ok = rf::mbar_wait<true>(&s.v_last, partial++ & 1, &s.abort, rf::kErrAttnWait);
             if (!__all_sync(0xffffffffu, ok)) return;
             if ((it.first + it.tiles - 1) * kTileN + row >= it.keys) {
                 uint8_t* at = ring + ((use - 2 + (uint32_t)(row >> 6)) % kStages) * kStageBytes + (row & 63) * 128;
@@ -605,7 +609,7 @@ __device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, u
             }
             rf::fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) rf::mbar_arrive_remote(rf::map_rank(rf::smem_addr(&s.v_clean), 0));
+            if (lane == 0) rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.v_clean), 0));
         }
         bool ok = rf::mbar_wait(&s.o_full, done & 1, &s.abort, rf::kErrAttnWait);
         if (ok) ok = rf::mbar_wait(&s.sum_full[done % 3], (done / 3) & 1, &s.abort, rf::kErrAttnWait);

@@ -72,8 +72,20 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
+/* kCluster: acquires what the arriving threads of the cluster's other CTAs released too (mbar_arrive_cluster). */
+template <bool kCluster = false>
 __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
     uint32_t done;
+    if constexpr (kCluster) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}\n"
+            : "=r"(done)
+            : "r"(smem_addr(bar)), "r"(parity)
+            : "memory");
+        return done != 0;
+    }
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
@@ -85,8 +97,19 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 }
 
 /* mbar_try_wait without the hardware's suspension: for lanes that watch different barriers. */
+template <bool kCluster = false>
 __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
     uint32_t done;
+    if constexpr (kCluster) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}\n"
+            : "=r"(done)
+            : "r"(smem_addr(bar)), "r"(parity)
+            : "memory");
+        return done != 0;
+    }
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
@@ -98,11 +121,12 @@ __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
 }
 
 /* A warp's wait for the barriers its lanes name (each its own phase), bounded and recorded as mbar_wait. */
+template <bool kCluster = false>
 __device__ __forceinline__ bool mbar_wait_lanes(uint64_t* bar, uint32_t parity, volatile int* abort, int err) {
-    if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
+    if (__all_sync(0xffffffffu, mbar_test_wait<kCluster>(bar, parity))) return true;
     const uint64_t t0 = global_ns();
     for (uint32_t i = 1;; ++i) {
-        if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
+        if (__all_sync(0xffffffffu, mbar_test_wait<kCluster>(bar, parity))) return true;
         if ((i & 255) == 0) {
             const bool late = global_ns() - t0 > kWaitTimeoutNs;
             if (__any_sync(0xffffffffu, *abort != 0 || late)) {
@@ -118,11 +142,12 @@ __device__ __forceinline__ bool mbar_wait_lanes(uint64_t* bar, uint32_t parity, 
 
 /* Wait for the phase of `bar` with parity `parity`; false (and *abort raised, the error recorded)
  * after the timeout, or at once when another role already raised *abort. */
+template <bool kCluster = false>
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int err) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (mbar_try_wait<kCluster>(bar, parity)) return true;
     const uint64_t t0 = global_ns();
     for (uint32_t i = 1;; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
+        if (mbar_try_wait<kCluster>(bar, parity)) return true;
         if ((i & 63) == 0) {
             if (*abort) return false;
             if (global_ns() - t0 > kWaitTimeoutNs) {
@@ -311,12 +336,6 @@ __device__ __forceinline__ void cluster_sync_all() {
 /* Arrive (release, cluster scope) on an mbarrier given by its shared::cluster address, in any CTA of the cluster. */
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t caddr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(caddr) : "memory");
-}
-
-/* The same arrival ordering only what this thread wrote within its own CTA (release at CTA scope, without the fence over the
- * cluster that costs about a microsecond): for hand-overs whose data the reader takes from the arriving CTA's memory. */
-__device__ __forceinline__ void mbar_arrive_remote(uint32_t caddr) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(caddr) : "memory");
 }
 
 /* Packed f32x2 arithmetic (sm_100): two lanes of f32 per instruction, each rounded as its scalar form. */

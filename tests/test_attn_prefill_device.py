@@ -410,3 +410,23 @@ def test_nan_in_a_split_call(cuda, product_lib, nq, nk, hq, hkv):
         assert torch.isnan(d["o"][:nq[0], group:2 * group]).all(), (first, last)
         d["o"][:nq[0], group:2 * group] = want[:nq[0], group:2 * group]
         assert torch.equal(d["o"], want)
+
+
+@pytest.mark.parametrize("nq,nk", [([37] * 60, [37] * 60), ([70, 1, 129] * 30, [200, 1, 129] * 30), ([30] * 3, [9001, 77, 3])])
+def test_sequence_ends_beside_nan_values(cuda, product_lib, nq, nk):
+    """Last key tiles that hold rows of other sequences, which a CTA clears before the pair's product reads them: the odd
+    sequences' v NaN, the even ones' answers finite, within their bounds and bit for bit the same a hundred times."""
+    torch = cuda
+    d = inputs(torch, 71, nq, nk, 16, 2, pad=3)
+    odd = torch.zeros(d["v"].shape[0], dtype=torch.bool, device="cuda")
+    rows = torch.zeros(d["q"].shape[0], dtype=torch.bool, device="cuda")
+    for i in range(len(nq)):
+        (rows[d["cu_q"][i]:d["cu_q"][i + 1]] if i % 2 == 0 else odd[d["cu_k"][i]:d["cu_k"][i + 1]])[:] = True
+    clean = dict(d, o=d["o"].clone())
+    assert call(product_lib, torch, clean) == abi.OK
+    check(torch, clean, heads=[0, 15])
+    d["v"][odd] = float("nan")
+    for _ in range(100):
+        d["o"].fill_(7.0)
+        assert call(product_lib, torch, d) == abi.OK
+        assert torch.equal(d["o"][rows], clean["o"][rows])

@@ -106,6 +106,12 @@ int ridgefill_gdn_step_device(const RadArgs* a, RadStream s);
 int64_t ridgefill_attn_prefill_scratch(const RadArgs* a);
 int64_t ridgefill_attn_decode_scratch(const RadArgs* a);
 
+/* Failure-detection self-test, as ridgefill_wait_selftest: launches, on stream `s`, one kernel whose warp waits as the
+ * prompt attention's warps do, half of its lanes for a barrier phase that is complete and half for one that nothing
+ * completes. The wait gives up after its limit (2 s), records its code for ridgefill_device_error and answers alike in
+ * every lane: status[0 .. 31] (device memory) are 0. RAD_E_INVAL on a null pointer. */
+int ridgefill_attn_wait_selftest(int* status, RadStream s);
+
 #ifdef __cplusplus
 }
 #endif

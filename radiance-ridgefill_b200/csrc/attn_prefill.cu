@@ -307,8 +307,7 @@ __device__ void announce(const Plan& p, Order& order, Shared& s, int owner) {
             continue;
         }
         const int slot = k % kRing;
-        if (!rf::mbar_wait(&s.item_empty[slot], ((k / kRing) & 1) ^ 1, &s.abort, rf::kErrAttnWait)) return;
-        __syncwarp();
+        if (!rf::mbar_wait_warp(&s.item_empty[slot], ((k / kRing) & 1) ^ 1, &s.abort, rf::kErrAttnWait)) return;
         if (owner < 0) order.own.rows = -1;
         if (order.lane == max(owner, 0)) {
             s.item[slot] = order.own;
@@ -328,8 +327,7 @@ struct Items {
         const int slot = k % kRing;
         Item it = {};
         it.rows = -1;
-        const bool ok = rf::mbar_wait(&s.item_full[slot], (k / kRing) & 1, &s.abort, rf::kErrAttnWait);
-        if (__all_sync(0xffffffffu, ok)) it = s.item[slot];
+        if (rf::mbar_wait_warp(&s.item_full[slot], (k / kRing) & 1, &s.abort, rf::kErrAttnWait)) it = s.item[slot];
         __syncwarp();
         if (lane == 0) rf::mbar_arrive(&s.item_empty[slot]);
         ++k;
@@ -598,8 +596,7 @@ __device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, u
         uint16_t* const out = g.o + (int64_t)it.q0 * g.o_row + (int64_t)(it.head * p.group) * g.o_head;
         use += 4 * it.tiles;
         if ((it.first + it.tiles) * kTileN > it.keys) {   /* V rows of the last tile past the sequence: the last two stages, 64 rows each */
-            const bool ok = rf::mbar_wait<true>(&s.v_last, partial++ & 1, &s.abort, rf::kErrAttnWait);
-            if (!__all_sync(0xffffffffu, ok)) return;
+            if (!rf::mbar_wait_warp<true>(&s.v_last, partial++ & 1, &s.abort, rf::kErrAttnWait)) return;
             if ((it.first + it.tiles - 1) * kTileN + row >= it.keys) {
                 uint8_t* at = ring + ((use - 2 + (uint32_t)(row >> 6)) % kStages) * kStageBytes + (row & 63) * 128;
 #pragma unroll
@@ -611,9 +608,9 @@ __device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, u
             __syncwarp();
             if (lane == 0) rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.v_clean), 0));
         }
-        bool ok = rf::mbar_wait(&s.o_full, done & 1, &s.abort, rf::kErrAttnWait);
-        if (ok) ok = rf::mbar_wait(&s.sum_full[done % 3], (done / 3) & 1, &s.abort, rf::kErrAttnWait);
-        if (!__all_sync(0xffffffffu, ok)) return;
+        if (!rf::mbar_wait_warp(&s.o_full, done & 1, &s.abort, rf::kErrAttnWait) ||
+            !rf::mbar_wait_warp(&s.sum_full[done % 3], (done / 3) & 1, &s.abort, rf::kErrAttnWait))
+            return;
         rf::tc_fence_after();
         const float sum = s.sum[done % 3][0][row] + s.sum[done % 3][1][row];
         if (it.slot >= 0) {   /* a piece: a thread its row's sums, a column's 128 rows side by side */
@@ -884,6 +881,33 @@ bool head_map(CUtensorMap* map, const uint16_t* base, int64_t T, int64_t heads, 
 }
 
 }  // namespace
+
+namespace {
+
+/* A warp's wait of which half the lanes see their phase complete and half one that nothing completes. */
+__global__ void wait_selftest_kernel(int* status) {
+    __shared__ uint64_t bar;
+    __shared__ int abort;
+    const int lane = threadIdx.x;
+    if (lane == 0) {
+        rf::mbar_init(&bar, 1);
+        abort = 0;
+        rf::mbar_init_fence();
+    }
+    __syncwarp();
+    if (lane == 0) rf::mbar_arrive(&bar);
+    __syncwarp();
+    status[lane] = rf::mbar_wait_warp(&bar, lane < 16 ? 0 : 1, &abort, rf::kErrAttnWait) ? 1 : 0;
+}
+
+}  // namespace
+
+/* Failure detection without a fault: see include/ridgefill_serve.h. */
+extern "C" int ridgefill_attn_wait_selftest(int* status, RadStream s) {
+    if (!status) return RAD_E_INVAL;
+    wait_selftest_kernel<<<1, 32, 0, rf::as_stream(s)>>>(status);
+    return rf::launch_status();
+}
 
 /* This translation unit's copy of the device error word (sm100.cuh), for ridgefill_device_error. */
 namespace rf {

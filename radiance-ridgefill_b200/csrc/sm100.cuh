@@ -159,6 +159,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     }
 }
 
+/* A whole warp's wait for one phase: the same answer in every lane. Alone, the lanes of a wait that gives up may disagree (one
+ * sees the phase complete, another the limit or *abort), and a warp that then parts leaves some of them where nothing bounds the
+ * wait: at a barrier that the others never reach. */
+template <bool kCluster = false>
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int err) {
+    return __all_sync(0xffffffffu, mbar_wait<kCluster>(bar, parity, abort, err));
+}
+
 /* 2-D TMA tile load into shared memory, completing `bytes` on `bar`. (x, y): innermost coordinate
  * first, in elements. One destination CTA. */
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int32_t x, int32_t y) {

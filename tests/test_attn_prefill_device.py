@@ -430,3 +430,24 @@ def test_sequence_ends_beside_nan_values(cuda, product_lib, nq, nk):
         d["o"].fill_(7.0)
         assert call(product_lib, torch, d) == abi.OK
         assert torch.equal(d["o"][rows], clean["o"][rows])
+
+
+def test_a_wait_gives_up_for_the_whole_warp(cuda, product_lib):
+    """Failure detection without a fault: a wait that half of a warp's lanes see complete and half do not gives up after its
+    limit in all of them, records its code, and the same context then answers a prompt."""
+    import ctypes
+    torch = cuda
+    lib = product_lib.lib
+    lib.ridgefill_device_error(1)
+    fn = lib.ridgefill_attn_wait_selftest
+    fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+    assert fn(None, None) == abi.E_INVAL
+    status = torch.full((32,), 7, dtype=torch.int32, device="cuda")
+    assert fn(status.data_ptr(), torch.cuda.current_stream().cuda_stream) == abi.OK
+    torch.cuda.synchronize()
+    assert status.tolist() == [0] * 32
+    assert lib.ridgefill_device_error(1) == 0x401
+    assert lib.ridgefill_device_error(0) == 0
+    d = inputs(torch, 72, [130, 9], [130, 200], 16, 2)
+    assert call(product_lib, torch, d) == abi.OK
+    check(torch, d)

@@ -32,11 +32,14 @@ bool word_rows(const RadTensor* t) {
     return true;
 }
 
+/* The base is a multiple of the element's `bytes`: what a kernel reads or writes element by element. */
+bool aligned(const RadTensor* t, unsigned bytes) { return (uintptr_t)t->data % bytes == 0; }
+
 /* A slot index operand of `n` rows: i32 [n] or [n, >= 1], its last axis dense. */
 int slot_rows(const RadTensor* t, int64_t n, int64_t* pitch) {
     if (t->dtype != RAD_I32) return RAD_E_DTYPE;
     if ((t->rank != 1 && t->rank != 2) || t->shape[0] != n || (t->rank == 2 && t->shape[1] < 1)) return RAD_E_SHAPE;
-    if (t->shape[t->rank - 1] > 1 && t->stride[t->rank - 1] != 1) return RAD_E_STRIDE;
+    if ((t->shape[t->rank - 1] > 1 && t->stride[t->rank - 1] != 1) || !aligned(t, 4)) return RAD_E_STRIDE;
     *pitch = t->rank == 1 ? 1 : t->stride[0];
     return RAD_OK;
 }
@@ -172,7 +175,9 @@ extern "C" int ridgefill_attn_prefill_parse(const RadArgs* a, RidgeFillAttnPrefi
         !is(V, { K->shape[0], hkv, D }) || T > most || K->shape[0] > most)
         return RAD_E_SHAPE;
     if (CQ->rank != 1 || CQ->shape[0] < 1 || CQ->shape[0] > 1 << 24 || (CK && !is(CK, { CQ->shape[0] }))) return RAD_E_SHAPE;
-    if (!word_rows(Q) || !word_rows(K) || !word_rows(V) || !word_rows(O) || !packed(CQ) || (CK && !packed(CK))) return RAD_E_STRIDE;
+    if (!word_rows(Q) || !word_rows(K) || !word_rows(V) || !word_rows(O) || !packed(CQ) || (CK && !packed(CK)) || !aligned(CQ, 4) ||
+        (CK && !aligned(CK, 4)))
+        return RAD_E_STRIDE;
     for (const RadTensor* t : { Q, K, V })
         for (int i = 0; i < 2; ++i)
             if (t->shape[i] > 1 && (t->stride[i] <= 0 || t->stride[i] >= 1LL << 39)) return RAD_E_STRIDE;
@@ -222,7 +227,8 @@ extern "C" int ridgefill_attn_decode_parse(const RadArgs* a, RidgeFillAttnDecode
     if (!is(Q, { B, h, D }) || !is(O, { B, h, D }) || !is(L, { B })) return RAD_E_SHAPE;
     if (C->rank != 4 || !is(C, { 2, C->shape[1], hkv, D }) || C->shape[1] < 0 || C->shape[1] > 0x7fffffffLL) return RAD_E_SHAPE;
     if (T->rank != 2 || T->shape[0] != B || T->shape[1] < 0 || T->shape[1] > 0x7fffff00LL / page) return RAD_E_SHAPE;
-    if (!word_rows(Q) || !word_rows(C) || !word_rows(O) || !packed(L) || (T->shape[1] > 1 && T->stride[1] != 1))
+    if (!word_rows(Q) || !word_rows(C) || !word_rows(O) || !packed(L) || (T->shape[1] > 1 && T->stride[1] != 1) ||
+        !aligned(T, 4) || !aligned(L, 4))
         return RAD_E_STRIDE;
     g->q = (const uint16_t*)Q->data;
     g->q_row = Q->stride[0];
@@ -282,8 +288,8 @@ extern "C" int ridgefill_gdn_step_parse(const RadArgs* a, RidgeFillGdnStep* g) {
         return RAD_E_SHAPE;
     const bool small_head = dv > 1 && S->stride[2] != dk;   /* the plane's rows are not packed */
     if (!word_rows(Q) || !word_rows(K) || O->stride[2] != 1 || V->stride[2] != 1 || (hv > 1 && (G->stride[1] != 1 || Be->stride[1] != 1)) ||
-        S->stride[3] != 1 || small_head || (uintptr_t)S->data % 16 || (S->shape[0] > 1 && S->stride[0] % 4) ||
-        (hv > 1 && S->stride[1] % 4))
+        !aligned(V, 2) || !aligned(O, 2) || !aligned(G, 4) || !aligned(Be, 4) || S->stride[3] != 1 || small_head || !aligned(S, 16) ||
+        (S->shape[0] > 1 && S->stride[0] % 4) || (hv > 1 && S->stride[1] % 4))
         return RAD_E_STRIDE;
     g->q = (const uint16_t*)Q->data;
     g->q_row = Q->stride[0];

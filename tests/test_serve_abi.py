@@ -260,3 +260,22 @@ def test_rows_found_by_several_threads():
     assert second is not None and second.op == b"ridgefill_gdn_fill"
     assert got[0] is not None and got[0].op == b"ridgefill_gdn_step"
     assert lib.find_row("no_such_row", abi.DOMAIN_DEVICE) is None
+
+
+# An address no kernel can read or write: not a multiple of its element's size.
+UNALIGNED = [
+    ("ridgefill_attn_prefill", "cu_q", abi.I32, [4], 2), ("ridgefill_attn_prefill", "cu_k", abi.I32, [4], 1),
+    ("ridgefill_attn_decode", "block_table", abi.I32, [3, 5], 2), ("ridgefill_attn_decode", "kv_lens", abi.I32, [3], 3),
+    ("ridgefill_gdn_step", "v", abi.BF16, [3, 4, 128], 1), ("ridgefill_gdn_step", "o", abi.BF16, [3, 4, 128], 7),
+    ("ridgefill_gdn_step", "g", abi.F32, [3, 4], 2), ("ridgefill_gdn_step", "beta", abi.F32, [3, 4], 1),
+    ("ridgefill_gdn_step", "state_idx", abi.I32, [3], 2), ("ridgefill_gdn_step", "out_idx", abi.I32, [3], 2),
+]
+
+
+@pytest.mark.parametrize("op,name,dtype,shape,off", UNALIGNED)
+def test_unaligned_addresses(product_lib, op, name, dtype, shape, off):
+    """Refused, and one element behind an aligned one accepted."""
+    base = {"ridgefill_attn_prefill": prefill_case, "ridgefill_attn_decode": decode_case, "ridgefill_gdn_step": step_case}[op]()
+    for at, want in ((off, abi.E_STRIDE), (2 if dtype == abi.BF16 else 4, abi.OK)):
+        tensors = list((base | {name: T(dtype, shape, off=at)}).values())
+        assert S.parse(product_lib, op + "_parse", tensors, cold_params(op)) == want

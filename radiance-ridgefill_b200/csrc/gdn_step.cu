@@ -135,6 +135,7 @@ extern "C" int ridgefill_gdn_step_device(const RadArgs* a, RadStream s) {
     const int rc = ridgefill_gdn_step_parse(a, &g);
     if (rc != RAD_OK) return rc;
     if (g.B == 0) return RAD_OK;
+    if (g.B > 0x7fffffffLL / g.n_head_v) return RAD_E_SHAPE;   /* so that no product of extents below passes 64 bits */
     cudaStream_t stream = rf::as_stream(s);
     /* Several state rows a lane in flight stream best (256 rows of 32 heads: of 128, 161 us with 64-row CTAs, 208 with 16-row
      * ones; of 64, 48 us with 32-row ones, 77 with 16; of 32, 24 and 38); while a head an SM would leave SMs idle, 16-row CTAs

@@ -279,3 +279,17 @@ def test_unaligned_addresses(product_lib, op, name, dtype, shape, off):
     for at, want in ((off, abi.E_STRIDE), (2 if dtype == abi.BF16 else 4, abi.OK)):
         tensors = list((base | {name: T(dtype, shape, off=at)}).values())
         assert S.parse(product_lib, op + "_parse", tensors, cold_params(op)) == want
+
+
+HUGE = 3074457345618258603   # 6 of them are 2 past 2^64
+
+
+def test_step_extents_past_64_bits(product_lib):
+    """M times n_head_v is checked before it is a grid: extents whose product passes 64 bits are refused, not wrapped."""
+    row = product_lib.find_row("ridgefill_gdn_step", abi.DOMAIN_DEVICE)
+    for B, hv in ((6, HUGE), (1 << 33, 4), (2, 1 << 31)):
+        tensors = dict(q=T(abi.BF16, [B, 1, 128], [128, 128, 1]), k=T(abi.BF16, [B, 1, 128], [128, 128, 1]),
+                       v=T(abi.BF16, [B, hv, 128], [128, 128, 1]), g=T(abi.F32, [B, hv], [1, 1]), beta=T(abi.F32, [B, hv], [1, 1]),
+                       state=T(abi.F32, [5, hv, 128, 128], [1 << 14, 1 << 14, 128, 1]), state_idx=T(abi.I32, [B]),
+                       out_idx=abi.absent(), o=T(abi.BF16, [B, hv, 128], [128, 128, 1]))
+        assert product_lib.launch(row, list(tensors.values()), S.step_params(B, 1, hv)) == abi.E_SHAPE, (B, hv)

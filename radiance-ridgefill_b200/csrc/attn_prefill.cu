@@ -843,6 +843,7 @@ __global__ void __launch_bounds__(kTileM) join_kernel(const Plan p) {
  *   four times 300 over 3,000 61, 70 whole; eight times 128 over 1,200 41, 25 whole; 30 times 2 over 300 63, 14 whole: the
  *   split goes through the sequences one by one */
 constexpr int kLongKeys = 8192, kLongAverage = 4096, kLeast = 6;
+constexpr int64_t kMostItems = 0x3fffffff;   /* query tiles, counted in 32 bits with a turn of the pairs to spare */
 struct Shape {
     int group, tokens;
     int64_t items;      /* query tiles (of all kv heads) at most: a sequence's last one may be cut short */
@@ -854,7 +855,8 @@ Shape shape_of(const RidgeFillAttnPrefill& g) {
     Shape s;
     s.group = (int)(g.n_head / g.n_head_kv);
     s.tokens = kTileM / s.group;
-    s.items = (g.T / (2 * s.tokens) + g.n_seq) * g.n_head_kv;
+    const int64_t tiles = g.T / (2 * s.tokens) + g.n_seq;
+    s.items = g.n_head_kv > kMostItems / tiles ? kMostItems + 1 : tiles * g.n_head_kv;   /* a call with more is refused */
     s.pairs = rf::sm_count() / 2;
     const bool few = s.items < s.pairs && 2 * g.Tk * (s.pairs - s.items) >= (int64_t)kLeast * kTileN * s.pairs * (g.n_seq + 1);
     const bool two = s.items <= 2 * s.pairs && g.Tk >= kLongKeys && 2 * g.Tk >= (int64_t)kLongAverage * (g.n_seq + 1);
@@ -926,7 +928,7 @@ extern "C" int ridgefill_attn_prefill_device(const RadArgs* a, RadStream s) {
     const RidgeFillAttnPrefill& g = p.g;
     if (g.T == 0 || g.n_seq == 0) return RAD_OK;
     const Shape sh = shape_of(g);
-    if (sh.items > 0x3fffffffLL) return RAD_E_SHAPE;
+    if (sh.items > kMostItems) return RAD_E_SHAPE;
     if (sh.split && (!a->scratch || a->scratch_bytes < sh.bytes || (uintptr_t)a->scratch % 16)) return RAD_E_INVAL;
     p.group = sh.group;
     p.tokens = sh.tokens;

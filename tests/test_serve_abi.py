@@ -293,3 +293,15 @@ def test_step_extents_past_64_bits(product_lib):
                        state=T(abi.F32, [5, hv, 128, 128], [1 << 14, 1 << 14, 128, 1]), state_idx=T(abi.I32, [B]),
                        out_idx=abi.absent(), o=T(abi.BF16, [B, hv, 128], [128, 128, 1]))
         assert product_lib.launch(row, list(tensors.values()), S.step_params(B, 1, hv)) == abi.E_SHAPE, (B, hv)
+
+
+def test_prefill_extents_past_64_bits(product_lib):
+    """The query tiles of all kv heads are counted without wrapping: too many of them are refused, and need no workspace."""
+    row = product_lib.find_row("ridgefill_attn_prefill", abi.DOMAIN_DEVICE)
+    for T_, h, n in ((1280, HUGE, 1), (40, 1 << 62, 1), (256, 1 << 29, 3)):
+        tensors = dict(q=T(abi.BF16, [T_, h, 256], [256, 256, 1]), k=T(abi.BF16, [1 << 20, h, 256], [256, 256, 1]),
+                       v=T(abi.BF16, [1 << 20, h, 256], [256, 256, 1]), cu_q=T(abi.I32, [n + 1]), cu_k=T(abi.I32, [n + 1]),
+                       o=T(abi.BF16, [T_, h, 256], [256, 256, 1]))
+        params = S.prefill_params(T_, h, h)
+        assert product_lib.scratch_bytes(row, list(tensors.values()), params) == 0
+        assert product_lib.launch(row, list(tensors.values()), params) == abi.E_SHAPE, (T_, h)

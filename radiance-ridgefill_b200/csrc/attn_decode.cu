@@ -595,9 +595,15 @@ int launch(const Plan& p, bool split, cudaStream_t s) {
 
 }  // namespace
 
+/* Heads (the join's grid) and the units of all items fit 32 bits; others are refused, before their products are formed. */
+static bool fits(const RidgeFillAttnDecode& g) {
+    if (g.B > 0x7fffffffLL / g.n_head) return false;
+    return g.B * g.n_head_kv * shape_of(g).chunks * (g.n_pages * g.page / kBlock + 1 + kStart) <= 0x7fffffffLL;
+}
+
 extern "C" int64_t ridgefill_attn_decode_scratch(const RadArgs* a) {
     RidgeFillAttnDecode g;
-    return ridgefill_attn_decode_parse(a, &g) == RAD_OK && g.B > 0 ? shape_of(g).bytes : 0;
+    return ridgefill_attn_decode_parse(a, &g) == RAD_OK && g.B > 0 && fits(g) ? shape_of(g).bytes : 0;
 }
 
 extern "C" int ridgefill_attn_decode_device(const RadArgs* a, RadStream s) {
@@ -605,10 +611,8 @@ extern "C" int ridgefill_attn_decode_device(const RadArgs* a, RadStream s) {
     const int rc = ridgefill_attn_decode_parse(a, &p.g);
     if (rc != RAD_OK) return rc;
     if (p.g.B == 0) return RAD_OK;
-    /* grids, and the units of all items, in 32 bits */
-    if (p.g.B > 0x7fffffffLL / p.g.n_head) return RAD_E_SHAPE;
+    if (!fits(p.g)) return RAD_E_SHAPE;
     const Shape sh = shape_of(p.g);
-    if (p.g.B * p.g.n_head_kv * sh.chunks * (p.g.n_pages * p.g.page / kBlock + 1 + kStart) > 0x7fffffffLL) return RAD_E_SHAPE;
     if (sh.split && (!a->scratch || a->scratch_bytes < sh.bytes || (uintptr_t)a->scratch % 16)) return RAD_E_INVAL;
     p.group = (int)(p.g.n_head / p.g.n_head_kv);
     p.chunks = sh.chunks;

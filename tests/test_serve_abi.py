@@ -305,3 +305,14 @@ def test_prefill_extents_past_64_bits(product_lib):
         params = S.prefill_params(T_, h, h)
         assert product_lib.scratch_bytes(row, list(tensors.values()), params) == 0
         assert product_lib.launch(row, list(tensors.values()), params) == abi.E_SHAPE, (T_, h)
+
+
+def test_decode_scratch_of_a_refused_call(product_lib):
+    """Extents that the call refuses need no workspace; their products are not formed."""
+    row = product_lib.find_row("ridgefill_attn_decode", abi.DOMAIN_DEVICE)
+    for B, h in ((3, HUGE * 2), (1 << 30, 1 << 40)):
+        tensors = dict(q=T(abi.BF16, [B, h, 256], [256, 256, 1]), kv_cache=T(abi.BF16, [2, 400, h, 256], [256, 256, 256, 1]),
+                       block_table=T(abi.I32, [B, 64]), kv_lens=T(abi.I32, [B]), o=T(abi.BF16, [B, h, 256], [256, 256, 1]))
+        params = S.decode_params(B, h, h, 16)
+        assert product_lib.launch(row, list(tensors.values()), params) == abi.E_SHAPE
+        assert product_lib.scratch_bytes(row, list(tensors.values()), params) == 0

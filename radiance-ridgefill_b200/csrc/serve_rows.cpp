@@ -44,11 +44,12 @@ int slot_rows(const RadTensor* t, int64_t n, int64_t* pitch) {
     return RAD_OK;
 }
 
-/* The optional `scale` parameter: 1 / sqrt(d) unless given; false when it is not a finite number (`positive`: above 0). */
+/* The optional `scale` parameter: 1 / sqrt(d) unless given; false when it is not a finite number (`positive`: above 0, and
+ * finite in the attention kernels' powers of two). */
 bool scale_of(const RadArgs* a, int64_t d, bool positive, float* out) {
     const double s = rad_args_getf_or(a, "scale", 1.0 / std::sqrt((double)d));
     *out = (float)s;
-    return std::isfinite(*out) && (*out > 0.0f || !positive);
+    return std::isfinite(*out) && (!positive || (*out > 0.0f && std::isfinite(*out * 1.4426950408889634f)));
 }
 
 /* ------------------------------------------------------------------ schemas */

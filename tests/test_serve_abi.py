@@ -316,3 +316,11 @@ def test_decode_scratch_of_a_refused_call(product_lib):
         params = S.decode_params(B, h, h, 16)
         assert product_lib.launch(row, list(tensors.values()), params) == abi.E_SHAPE
         assert product_lib.scratch_bytes(row, list(tensors.values()), params) == 0
+
+
+@pytest.mark.parametrize("op,case", [("ridgefill_attn_prefill", prefill_case), ("ridgefill_attn_decode", decode_case)])
+def test_scales_that_overflow(product_lib, op, case):
+    """The kernels work in powers of two: a scale whose product with log2(e) is no finite f32 is refused."""
+    for scale, want in ((3e38, abi.E_INVAL), (2.4e38, abi.E_INVAL), (2.3e38, abi.OK), (1e-30, abi.OK), (1e-60, abi.E_INVAL)):
+        params = cold_params(op) + [H.pf64("scale", scale)]
+        assert S.parse(product_lib, op + "_parse", list(case().values()), params) == want, scale

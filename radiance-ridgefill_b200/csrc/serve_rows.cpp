@@ -171,9 +171,9 @@ extern "C" int ridgefill_attn_prefill_parse(const RadArgs* a, RidgeFillAttnPrefi
         return RAD_E_DTYPE;
     if (T < 0 || h <= 0 || hkv <= 0) return RAD_E_SHAPE;
     if (h % hkv != 0 || h / hkv > 128) return RAD_E_UNSUPPORTED;
-    const int64_t most = 0x7ffffe00LL;   /* rows, with a tile's to spare, in 32 bits */
+    const int64_t most = 0x7ffffe00LL;   /* rows and keys together, with a tile's to spare, in 32 bits */
     if (!is(Q, { T, h, D }) || !is(O, { T, h, D }) || K->rank != 3 || !is(K, { K->shape[0], hkv, D }) || K->shape[0] < 0 ||
-        !is(V, { K->shape[0], hkv, D }) || T > most || K->shape[0] > most)
+        !is(V, { K->shape[0], hkv, D }) || T > most || K->shape[0] > most - T)
         return RAD_E_SHAPE;
     if (CQ->rank != 1 || CQ->shape[0] < 1 || CQ->shape[0] > 1 << 24 || (CK && !is(CK, { CQ->shape[0] }))) return RAD_E_SHAPE;
     if (!word_rows(Q) || !word_rows(K) || !word_rows(V) || !word_rows(O) || !packed(CQ) || (CK && !packed(CK)) || !aligned(CQ, 4) ||

@@ -324,3 +324,11 @@ def test_scales_that_overflow(product_lib, op, case):
     for scale, want in ((3e38, abi.E_INVAL), (2.4e38, abi.E_INVAL), (2.3e38, abi.OK), (1e-30, abi.OK), (1e-60, abi.E_INVAL)):
         params = cold_params(op) + [H.pf64("scale", scale)]
         assert S.parse(product_lib, op + "_parse", list(case().values()), params) == want, scale
+
+
+def test_prefill_rows_and_keys_in_32_bits(product_lib):
+    """A query tile's last key is reckoned from rows and keys together, in 32 bits: both at their most are refused."""
+    for rows, keys, want in ((1 << 30, 0x7ffffe00, abi.E_SHAPE), (1 << 30, (1 << 30) - 512, abi.OK), (1 << 30, (1 << 30) - 511, abi.E_SHAPE),
+                             (40, 0x7ffffe00 - 40, abi.OK), (40, 0x7ffffe00 - 39, abi.E_SHAPE)):
+        tensors = list(prefill_case(T_=rows, keys=keys, hq=2).values())
+        assert S.parse(product_lib, "ridgefill_attn_prefill_parse", tensors, S.prefill_params(rows, 2, 2)) == want, (rows, keys)

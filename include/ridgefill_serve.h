@@ -35,7 +35,7 @@ enum { GS_Q = 0, GS_K, GS_V, GS_G, GS_BETA, GS_STATE, GS_STATE_IDX, GS_OUT_IDX, 
  * products summed in f32; p is rounded to bf16 for the product with v and summed in f32; o is rounded once. A value of v
  * that is not finite reaches the rows that see it and may reach earlier rows of its own sequence, those whose last key lies
  * up to 126 + 256 / (Hq / Hkv) before it (they share a query tile and a key tile with rows that see its neighbours, and
- * their weight for it is zero); no row of another sequence. */
+ * their weight for it is zero); no row that sees no key, and no row of another sequence. */
 typedef struct RidgeFillAttnPrefill {
     const uint16_t* q;       int64_t q_row, q_head;              /* [T, Hq, D] */
     const uint16_t* k;       int64_t k_row, k_head;              /* [Tk, Hkv, D] */

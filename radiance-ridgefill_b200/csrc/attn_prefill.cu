@@ -660,6 +660,10 @@ __device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, u
                 }
                 *(uint4*)(tile + lane * 128 + ((v ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
+            if (inv == 0.f) {   /* again: where the tile's V is not finite, zero weights have left a NaN in O */
+#pragma unroll 1
+                for (int v = 0; v < 8; ++v) *(uint4*)(tile + lane * 128 + (v << 4)) = make_uint4(0u, 0u, 0u, 0u);
+            }
             __syncwarp();
             uint4 t[8];
 #pragma unroll

@@ -451,3 +451,23 @@ def test_a_wait_gives_up_for_the_whole_warp(cuda, product_lib):
     d = inputs(torch, 72, [130, 9], [130, 200], 16, 2)
     assert call(product_lib, torch, d) == abi.OK
     check(torch, d)
+
+
+@pytest.mark.parametrize("nq,nk,hq,hkv", [([53], [17], 16, 2), ([300, 20], [100, 20], 8, 1), ([40] * 40, [3] * 40, 4, 1), ([129], [128], 128, 1),
+                                          ([20, 64], [9000, 10], 16, 2), ([10, 40, 700], [9000, 1, 650], 16, 2)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_rows_without_keys_beside_values_that_are_not_finite(cuda, product_lib, nq, nk, hq, hkv, value):
+    """A row that sees no key is zero, whatever its sequence's keys, values and other rows hold; whole query tiles and split
+    calls."""
+    torch = cuda
+    d = inputs(torch, 73, nq, nk, hq, hkv)
+    clean = dict(d, o=d["o"].clone())
+    assert call(product_lib, torch, clean) == abi.OK
+    check(torch, clean, heads=[0, hq - 1])
+    empty = [(q0, max(a - b, 0)) for q0, a, b in zip(d["cu_q"], nq, nk)]
+    for name in ("v", "k", "q"):
+        d[name][:] = value
+        d["o"].fill_(7.0)
+        assert call(product_lib, torch, d) == abi.OK
+        for q0, n in empty:
+            assert (d["o"][q0:q0 + n] == 0).all(), name

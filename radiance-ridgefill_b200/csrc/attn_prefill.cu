@@ -21,10 +21,12 @@
  *               exponentials, sums, P. The running maximum is followed only when a tile exceeds it by 2^8: rescaling O,
  *               256 columns of tensor memory a row, is then rare, and the weights of a row stay below 2^8
  *   warps 8-11  the output: O from tensor memory, divided by the row's sum, rounded once to bf16, turned in shared memory
- *               so that eight lanes write 128 bytes of a row, while the next query tile's products run; and, where a
- *               sequence's last key tile is not full, the zeroing of its V rows past the end (another sequence's rows, or
- *               anything behind the last one: P is zero there, but a NaN times zero is not)
+ *               so that eight lanes write 128 bytes of a row, while the next query tile's products run
  *   warp 12     TMA loads     warp 13  the products' issue (the pair's first CTA)     warp 14  the order of the tiles
+ *   warp 15     where a sequence's last key tile is not full, the zeroing of its V rows past the end (another sequence's
+ *               rows, or anything behind the last one: P is zero there, but a NaN times zero is not). Its release to the
+ *               pair's first CTA waits for all that the warp has under way; a warp of its own has nothing (released by the
+ *               output's warps, behind their stores, 60 prompts of 37 rows took 27.5 us, 21.9 so)
  * P as bf16 costs half a bf16 step a weight, of the order of the output's own rounding; f32 elsewhere.
  *
  * Measured, 16 query heads over 2: 16,384 rows 1,364 us (1.61 PFLOP/s; the tensor pipe is active 89 % of the SMs' time),
@@ -44,7 +46,7 @@ namespace {
 constexpr int D = 256, kTileM = 128, kTileN = 128;           /* rows of a CTA (the pair's tile has 256); keys */
 constexpr int kStages = 8, kStageBytes = 16384, kQBytes = kTileM * D * 2;
 constexpr int kBoxBytes = 64 * 64 * 2;                       /* one TMA box of K or V: 64 rows x 64 elements */
-constexpr int kSoftWarps = 8, kOutWarps = 4, kWarps = kSoftWarps + kOutWarps + 3, kThreads = 32 * kWarps;
+constexpr int kSoftWarps = 8, kOutWarps = 4, kWarps = kSoftWarps + kOutWarps + 4, kThreads = 32 * kWarps;
 constexpr int kTurnBytes = 32 * 128;                         /* an output warp's 32 rows x 64 elements */
 constexpr int kRing = 4;                                     /* query tiles announced ahead */
 constexpr uint32_t kTmemCols = 512, kColO = 256;
@@ -74,6 +76,9 @@ struct Item {
     int q0, rows, k0, keys, first, tiles, limit, head, slot;
 };
 
+/* Whether the item's last key tile is not full: its V rows past the sequence are zeroed before the product reads them. */
+__device__ __forceinline__ bool cut_short(const Item& it) { return (it.first + it.tiles) * kTileN > it.keys; }
+
 struct Shared {
     Item item[kRing];
     int64_t at[kTileM];                    /* where row r of the CTA's lies in o, from the first one's place */
@@ -82,7 +87,7 @@ struct Shared {
     float sum[3][2][kTileM];               /* rows' sums (two halves) of the query tiles under way */
     uint64_t item_full[kRing], item_empty[kRing];
     uint64_t q_full, q_empty, kv_full[kStages], kv_empty[kStages];
-    uint64_t s_full[2], p_full[2], pv_done[2], v_last, v_clean, o_full, o_empty, sum_full[3], drain;
+    uint64_t s_full[2], p_full[2], pv_done[2], v_land[2], v_clean[2], o_full, o_empty, sum_full[3], drain;
     uint32_t tmem;
     int abort;
 };
@@ -337,23 +342,32 @@ struct Items {
 
 /* ------------------------------------------------------------------ roles */
 
-/* Both CTAs of the pair; the bytes of both complete on the first CTA's barriers. */
+/* Both CTAs of the pair; the bytes of both complete on the first CTA's barriers, but for the V rows of a key tile cut short:
+ * those complete in their own CTA (v_land), where they are zeroed past the sequence before v_clean tells the products. */
 __device__ void produce(const Plan& p, Shared& s, uint8_t* qtile, uint8_t* ring, const CUtensorMap* map_q, const CUtensorMap* map_k,
                         const CUtensorMap* map_v, int rank, int lane) {
     Items items{ s };
-    uint32_t use = 0, done = 0;   /* stages filled; query tiles with keys */
+    uint32_t use = 0, done = 0, partial = 0;   /* stages filled; query tiles with keys; those cut short */
     const uint32_t q_bytes = 2u * 4u * (uint32_t)(p.group * p.tokens) * 128u;
     bool ok = true;
     for (;;) {
         const Item it = items.next(lane);
         if (it.rows < 0) break;
         if (lane == 0 && ok) {
-            /* a stage: 64 rows of two 64-element columns from element x */
-            auto stage = [&](const CUtensorMap* map, int x, int row) {
+            /* a stage: 64 rows of two 64-element columns from element x. land 0, 1: the first and second of a V cut short */
+            auto stage = [&](const CUtensorMap* map, int x, int row, int land) {
                 if (ok) ok = rf::mbar_wait(&s.kv_empty[use % kStages], ((use / kStages) & 1) ^ 1, &s.abort, rf::kErrAttnWait);
                 if (!ok) return;
-                const uint32_t st = use % kStages, bar = rf::map_rank(rf::smem_addr(&s.kv_full[st]), 0);
-                if (rank == 0) rf::mbar_arrive_expect_tx(&s.kv_full[st], 2 * kStageBytes);
+                const uint32_t st = use % kStages;
+                uint32_t bar;
+                if (land < 0) {
+                    bar = rf::map_rank(rf::smem_addr(&s.kv_full[st]), 0);
+                    if (rank == 0) rf::mbar_arrive_expect_tx(&s.kv_full[st], 2 * kStageBytes);
+                } else {
+                    bar = rf::map_rank(rf::smem_addr(&s.v_land[partial & 1]), rank);
+                    if (land == 0) rf::mbar_arrive_expect_tx(&s.v_land[partial & 1], 2 * kStageBytes);   /* both stages' */
+                    if (rank == 0) rf::mbar_arrive(&s.kv_full[st]);
+                }
                 rf::tma_load_3d_pair(ring + st * kStageBytes, map, bar, x, it.head, row);
                 rf::tma_load_3d_pair(ring + st * kStageBytes + kBoxBytes, map, bar, x + 64, it.head, row);
                 ++use;
@@ -368,10 +382,12 @@ __device__ void produce(const Plan& p, Shared& s, uint8_t* qtile, uint8_t* ring,
             }
             for (int j = 0; j <= it.tiles; ++j) {
                 if (j < it.tiles)   /* this CTA's 64 keys of the tile */
-                    for (int h = 0; h < 2; ++h) stage(map_k, h * 128, it.k0 + (it.first + j) * kTileN + rank * 64);
+                    for (int h = 0; h < 2; ++h) stage(map_k, h * 128, it.k0 + (it.first + j) * kTileN + rank * 64, -1);
                 if (j > 0)          /* the tile's keys, this CTA's 128 elements */
-                    for (int h = 0; h < 2; ++h) stage(map_v, rank * 128, it.k0 + (it.first + j - 1) * kTileN + h * 64);
+                    for (int h = 0; h < 2; ++h)
+                        stage(map_v, rank * 128, it.k0 + (it.first + j - 1) * kTileN + h * 64, j == it.tiles && cut_short(it) ? h : -1);
             }
+            partial += cut_short(it);
         }
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
         if (!ok) break;
@@ -442,20 +458,14 @@ __device__ void multiply(Shared& s, const uint8_t* qtile, const uint8_t* ring, u
             use += 2;
         }
         if (j >= 0) {
-            const bool last = j + 1 == it.tiles, cut = last && (it.first + it.tiles) * kTileN > it.keys;
-            if (cut) {   /* the last V rows have landed: those past the sequence may be cleared, in both CTAs */
-                const uint32_t u = v + (lane & 1);   /* the copies of both CTAs complete here: acquired and released at cluster scope */
-                ok = rf::mbar_wait_lanes<true>(full(u), phase(u), &s.abort, rf::kErrAttnWait);
-                if (!ok) break;
-                if (lane < 2) rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.v_last), lane));
-                __syncwarp();
-            }
+            const bool last = j + 1 == it.tiles, cut = last && cut_short(it);
             uint64_t* p = &s.p_full[tile & 1];
             const uint32_t pp = (tile >> 1) & 1;
             if (!wait(p, pp, full(v), phase(v), full(v + 1), phase(v + 1), j == 0 ? &s.o_empty : p, j == 0 ? (done & 1) ^ 1 : pp)) break;
-            if (cut) {   /* the zeros of both CTAs, before the product that reads them */
-                ok = rf::mbar_wait_lanes<true>(&s.v_clean, partial++ & 1, &s.abort, rf::kErrAttnWait);
+            if (cut) {   /* V of both CTAs, landed and zeroed past the sequence */
+                ok = rf::mbar_wait_lanes<true>(&s.v_clean[partial & 1], (partial >> 1) & 1, &s.abort, rf::kErrAttnWait);
                 if (!ok) break;
+                ++partial;
             }
             const uint32_t a = tmem + (tile & 1) * kTileN;
 #pragma unroll
@@ -583,10 +593,33 @@ __device__ void soften(const Plan& p, Shared& s, uint32_t tmem, int warp, int la
     }
 }
 
-__device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, uint32_t tmem, int rank, int warp, int lane) {
+/* V's rows past the sequence in a last key tile cut short, zeroed in this CTA's memory. Two barriers in turn: the ring holds V
+ * of two such tiles at most, the third one's first stage being the first one's, which the product has read by then. */
+__device__ void clean(Shared& s, uint8_t* ring, int lane) {
+    Items items{ s };
+    uint32_t use = 0, partial = 0;
+    for (;;) {
+        const Item it = items.next(lane);
+        if (it.rows < 0) return;
+        use += 4 * it.tiles;   /* the last two stages: 64 rows of V each */
+        if (!cut_short(it)) continue;
+        if (!rf::mbar_wait_warp(&s.v_land[partial & 1], (partial >> 1) & 1, &s.abort, rf::kErrAttnWait)) return;
+        /* a row's 128 bytes in each of the stage's two boxes; two rows an instruction */
+        const int first = it.keys - (it.first + it.tiles - 1) * kTileN;
+        for (int row = first + (lane >> 4); row < kTileN; row += 2)
+            *(uint4*)(ring + ((use - 2 + (uint32_t)(row >> 6)) % kStages) * kStageBytes + (lane >> 3 & 1) * kBoxBytes + (row & 63) * 128 +
+                      (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        rf::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.v_clean[partial & 1]), 0));
+        ++partial;
+    }
+}
+
+__device__ void output(const Plan& p, Shared& s, uint8_t* turn, uint32_t tmem, int rank, int warp, int lane) {
     const RidgeFillAttnPrefill& g = p.g;
     Items items{ s };
-    uint32_t use = 0, done = 0, partial = 0;
+    uint32_t done = 0;
     const int row = warp * 32 + lane;
     const uint32_t mine = tmem + kColO + ((uint32_t)(warp * 32) << 16);
     for (;;) {
@@ -594,20 +627,6 @@ __device__ void output(const Plan& p, Shared& s, uint8_t* ring, uint8_t* turn, u
         if (it.rows < 0) return;
         const int live = it.rows * p.group;   /* this CTA's rows */
         uint16_t* const out = g.o + (int64_t)it.q0 * g.o_row + (int64_t)(it.head * p.group) * g.o_head;
-        use += 4 * it.tiles;
-        if ((it.first + it.tiles) * kTileN > it.keys) {   /* V rows of the last tile past the sequence: the last two stages, 64 rows each */
-            if (!rf::mbar_wait_warp<true>(&s.v_last, partial++ & 1, &s.abort, rf::kErrAttnWait)) return;
-            if ((it.first + it.tiles - 1) * kTileN + row >= it.keys) {
-                uint8_t* at = ring + ((use - 2 + (uint32_t)(row >> 6)) % kStages) * kStageBytes + (row & 63) * 128;
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) *(uint4*)(at + b * kBoxBytes + c * 16) = make_uint4(0u, 0u, 0u, 0u);
-            }
-            rf::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) rf::mbar_arrive_cluster(rf::map_rank(rf::smem_addr(&s.v_clean), 0));
-        }
         if (!rf::mbar_wait_warp(&s.o_full, done & 1, &s.abort, rf::kErrAttnWait) ||
             !rf::mbar_wait_warp(&s.sum_full[done % 3], (done / 3) & 1, &s.abort, rf::kErrAttnWait))
             return;
@@ -707,8 +726,10 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             rf::mbar_init(&s.p_full[i], 2 * kSoftWarps);   /* first CTA's: both CTAs' warps */
             rf::mbar_init(&s.pv_done[i], 1);
         }
-        rf::mbar_init(&s.v_last, 1);
-        rf::mbar_init(&s.v_clean, 2 * kOutWarps);
+        for (int i = 0; i < 2; ++i) {
+            rf::mbar_init(&s.v_land[i], 1);    /* each CTA's: its producer, its bytes */
+            rf::mbar_init(&s.v_clean[i], 2);   /* first CTA's: both CTAs' zeroing warps */
+        }
         rf::mbar_init(&s.o_full, 1);
         rf::mbar_init(&s.o_empty, 2 * kOutWarps);
         for (int i = 0; i < 3; ++i) rf::mbar_init(&s.sum_full[i], kSoftWarps);
@@ -745,8 +766,9 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     rf::tc_fence_after();
     const uint32_t tmem = s.tmem;
     if (warp < 8) soften(p, s, tmem, warp, lane);
-    else if (warp < 12) output(p, s, ring, turn, tmem, rank, warp - 8, lane);
+    else if (warp < 12) output(p, s, turn, tmem, rank, warp - 8, lane);
     else if (warp == 12) produce(p, s, qtile, ring, &map_q, &map_k, &map_v, rank, lane);
+    else if (warp == 15) clean(s, ring, lane);
     else if (rank == 0) multiply(s, qtile, ring, tmem, lane);
     rf::tc_fence_before();
     rf::cluster_sync_all();   /* no product reads the other CTA's memory any more */

@@ -841,9 +841,9 @@ __global__ void __launch_bounds__(kTileM) join_kernel(const Plan p) {
         for (int c = 0; c < kCols; ++c) acc[c] *= f;
 #pragma unroll
         for (int k = 0; k < kFlight; ++k) {
-            /* no piece, or none of its keys is the row's; with a NaN sum (the maximum passes over NaN scores) it goes on, so
-             * that the row is NaN as it is from whole query tiles */
-            if (ml[k].x == kNone && ml[k].y == 0.f) continue;
+            /* no piece, or none of its keys is the row's; by the sum, since a row of NaN scores has no maximum either (fmaxf
+             * passes over them), but a NaN sum, and is NaN as it is from whole query tiles */
+            if (ml[k].y == 0.f) continue;
             const float w = exp2_approx(ml[k].x - up);
             sum = fmaf(w, ml[k].y, sum);
 #pragma unroll

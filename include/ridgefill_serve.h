@@ -12,6 +12,7 @@
  * a graph. Values in device memory (lengths, page and slot numbers) are read where the kernel runs, with a fail-safe:
  * cu_seqlens and lengths are clamped into their operands, a page or slot outside its pool is not read or written.
  * A call's workspace is its own until the call has run: calls that may overlap on the GPU need one each.
+ * Every address is a multiple of its element's size at least (of 16 bytes where a row is read in words: the parses say where).
  * An operand with an extent of 0 still carries an address: one without it counts as not given.
  */
 #ifndef RIDGEFILL_SERVE_H
@@ -66,7 +67,9 @@ typedef struct RidgeFillAttnDecode {
  *     S <- exp(g[i, h]) S;  S <- S + beta[i, h] (v - S k) k^T;  o[i, h] = scale S q
  * the new S written to slot out_idx[i] (idx[i] without out_idx), in f32 throughout, o rounded once to bf16. A row is
  * skipped -- no state and no o written -- when one of its slots lies outside the pool, or when the slot it would
- * write is named by another row (written or read by it): rows that share a slot have no order among themselves. */
+ * write is named by another row (written or read by it): rows that share a slot have no order among themselves. To see
+ * that, all B slot numbers are read for every head of every row: meant for batches of hundreds of rows (at 4,096 rows of 32
+ * heads of 128 the call runs at 0.6 of its rate at 512). */
 typedef struct RidgeFillGdnStep {
     const uint16_t* q;       int64_t q_row, q_head;              /* [B, Hk, dk] */
     const uint16_t* k;       int64_t k_row, k_head;              /* [B, Hk, dk] */

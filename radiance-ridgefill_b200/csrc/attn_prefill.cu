@@ -10,7 +10,8 @@
  * A CTA's 128 rows are the 128 / group tokens' rows of all `group` query heads of one kv head, the pair's second CTA
  * taking the next tokens: a key tile is read once for the whole group, and the causal edge cuts at 2 x 128 / group rows,
  * not at 256. Persistent pairs take query tiles from the longest to the shortest, in turns that run back and forth, so
- * that their sums are near alike; few query tiles over long keys are split along the keys instead (Spans).
+ * that their sums are near alike (past 32 sequences in the batch's order: Order); few query tiles over long keys are split
+ * along the keys instead (Spans).
  *
  * Tensor memory (512 columns a CTA): two 128-column buffers of scores, and O's 256. P, rounded to bf16, replaces its
  * scores in place (64 columns) and is the second product's A operand from there. Shared memory: Q's 64 KiB and a ring of
@@ -167,7 +168,7 @@ __device__ __forceinline__ int lane_holding(int x, int at, int lane, int* before
  * span that holds all key tiles of a query tile writes its output; the at most two that it cuts leave Partials (slot 1 of
  * the pair that has the first of them, slot 0 of the others), which join_kernel adds up. */
 struct Spans {
-    int n, each, extra;   /* the first `extra` spans one longer; with few tiles fewer spans, of two at least */
+    int n, each, extra;   /* the first `extra` spans one longer; with few tiles fewer spans, of two, or one where that is odd */
     __device__ __forceinline__ Spans(int total, int most) {
         n = max(min((total + 1) / 2, most), 1);
         each = total / n;
@@ -198,7 +199,9 @@ __device__ __forceinline__ void walk(const Plan& p, int lane, F&& at) {
 
 /* The order of this pair's query tiles, the whole warp 14 of both CTAs, which reach the same order by themselves. Up to 32
  * sequences (a lane each) the tiles go from the most key tiles to the fewest over all sequences, in turns back and forth;
- * with more, in the batch's order. Split over the keys: the pieces of the pair's span. */
+ * with more, in the batch's order, which costs up to 15 %: 32 prompts of 1 to 500 rows 62 us sorted, 68 in their order, of 100
+ * to 2,048 406 and 402, of 256 and a last one of 4,096 134 and 154, of 64 to 2,048 falling 356 and 384. Split over the keys:
+ * the pieces of the pair's span. */
 struct Order {
     const Plan& p;
     int rank, lane, heads, pairs, pair, tokens;
@@ -867,7 +870,10 @@ __global__ void __launch_bounds__(kTileM) join_kernel(const Plan p) {
  *   with at most two a pair, keys from kLongKeys on and a sequence of twice the average from kLongAverage: 2,048 rows over
  *   32,768, 128 query tiles of 256 key tiles on 74 pairs, would take two rounds, 86 % of the pairs' time: 670 us, 704 whole;
  *   four times 300 over 3,000 61, 70 whole; eight times 128 over 1,200 41, 25 whole; 30 times 2 over 300 63, 14 whole: the
- *   split goes through the sequences one by one */
+ *   split goes through the sequences one by one
+ * The extents decide, which in a captured call may be much larger than the sequences of the moment: 2,048 rows over 2,048
+ * keys in operands of 32,768 keys 55 us, 34 in their own; 37 rows in 512 and 4,096 keys 16.6 and 10.5, 16 over 500 in 32,768
+ * 17.8 and 16.5 */
 constexpr int kLongKeys = 8192, kLongAverage = 4096, kLeast = 6;
 constexpr int64_t kMostItems = 0x3fffffff;   /* query tiles, counted in 32 bits with a turn of the pairs to spare */
 struct Shape {

@@ -10,6 +10,11 @@
  * words are loaded before the first is used. Loads and stores go through L2 alone, without the streaming hint, which cost
  * 3 % (169.8 -> 164.8 us at 256 rows of 32 heads). Four warps a CTA: 161 us, 6.70 TB/s, the measured copy rate and a little
  * more; 28.9 us at 27 rows of 48 heads (5.91 TB/s), 2.9 us at one row of 32.
+ *
+ * Every CTA looks through all rows' slot numbers for one that names the slot it writes, so that part grows with the square of
+ * the rows: nothing up to some 500 (512 rows of 32 heads of 128 6.84 TB/s), a few percent at 1,024 (6.27), a third at 4,096
+ * (4.04). Heads of up to 32 stay further from the memory's rate (256 rows of 32 heads 2.9 TB/s): a CTA moves 4 KiB each way, two
+ * words in flight a lane, for one look through the slots and one barrier; fewer and larger CTAs were not built.
  */
 #include <cuda_bf16.h>
 

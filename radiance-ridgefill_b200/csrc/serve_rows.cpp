@@ -121,8 +121,9 @@ int shape_step(const RadParam* p, int n_p, int operand, RadOpdDesc* out) {
 
 const RadKernelInfo kServeRows[] = {
     SERVE_ROW("ridgefill_attn_prefill_sm100", "ridgefill_attn_prefill",
-              "tcgen05 kind::f16 into tensor memory, TMA-fed: 128 rows (all query heads of a kv head side by side) x 128 keys a "
-              "tile, the weights back into tensor memory as the second product's operand, persistent CTAs, longest tiles first",
+              "tcgen05 kind::f16 over CTA pairs into tensor memory, TMA-fed: 2 x 128 rows (all query heads of a kv head side by "
+              "side) x 128 keys a tile, the weights back into tensor memory as the second product's operand; persistent pairs take "
+              "query tiles, longest first up to 32 sequences, else in the batch's order; few over long keys split and joined",
               "head_dim 256, up to 128 query heads a kv head", "bf16 q / k / v / o, i32 cu_seqlens / cu_keys",
               ridgefill_attn_prefill_device, ridgefill_attn_prefill_scratch, shape_prefill),
     SERVE_ROW("ridgefill_attn_decode_sm100", "ridgefill_attn_decode",

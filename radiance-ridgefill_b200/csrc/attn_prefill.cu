@@ -27,7 +27,7 @@
  *   warp 15     where a sequence's last key tile is not full, the zeroing of its V rows past the end (another sequence's
  *               rows, or anything behind the last one: P is zero there, but a NaN times zero is not). Its release to the
  *               pair's first CTA waits for all that the warp has under way; a warp of its own has nothing (released by the
- *               output's warps, behind their stores, 60 prompts of 37 rows took 27.5 us, 21.9 so)
+ *               output's warps, behind their stores, 60 prompts of 37 rows took 27.5 us, 21.9 so; one such prompt alone 10.3 both ways)
  * P as bf16 costs half a bf16 step a weight, of the order of the output's own rounding; f32 elsewhere.
  *
  * Measured, 16 query heads over 2: 16,384 rows 1,364 us (1.61 PFLOP/s; the tensor pipe is active 89 % of the SMs' time),
@@ -913,10 +913,6 @@ bool head_map(CUtensorMap* map, const uint16_t* base, int64_t T, int64_t heads, 
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-
-}  // namespace
-
-namespace {
 
 /* A warp's wait of which half the lanes see their phase complete and half one that nothing completes. */
 __global__ void wait_selftest_kernel(int* status) {

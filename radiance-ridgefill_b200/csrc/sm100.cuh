@@ -72,20 +72,8 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
-/* kCluster: acquires what the arriving threads of the cluster's other CTAs released too (mbar_arrive_cluster). */
-template <bool kCluster = false>
 __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
     uint32_t done;
-    if constexpr (kCluster) {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}\n"
-            : "=r"(done)
-            : "r"(smem_addr(bar)), "r"(parity)
-            : "memory");
-        return done != 0;
-    }
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
@@ -96,7 +84,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
     return done != 0;
 }
 
-/* mbar_try_wait without the hardware's suspension: for lanes that watch different barriers. */
+/* mbar_try_wait without the hardware's suspension: for lanes that watch different barriers. kCluster: acquires what the
+ * arriving threads of the cluster's other CTAs released too (mbar_arrive_cluster). */
 template <bool kCluster = false>
 __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
     uint32_t done;
@@ -142,12 +131,11 @@ __device__ __forceinline__ bool mbar_wait_lanes(uint64_t* bar, uint32_t parity, 
 
 /* Wait for the phase of `bar` with parity `parity`; false (and *abort raised, the error recorded)
  * after the timeout, or at once when another role already raised *abort. */
-template <bool kCluster = false>
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int err) {
-    if (mbar_try_wait<kCluster>(bar, parity)) return true;
+    if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = global_ns();
     for (uint32_t i = 1;; ++i) {
-        if (mbar_try_wait<kCluster>(bar, parity)) return true;
+        if (mbar_try_wait(bar, parity)) return true;
         if ((i & 63) == 0) {
             if (*abort) return false;
             if (global_ns() - t0 > kWaitTimeoutNs) {
@@ -162,9 +150,8 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
 /* A whole warp's wait for one phase: the same answer in every lane. Alone, the lanes of a wait that gives up may disagree (one
  * sees the phase complete, another the limit or *abort), and a warp that then parts leaves some of them where nothing bounds the
  * wait: at a barrier that the others never reach. */
-template <bool kCluster = false>
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int err) {
-    return __all_sync(0xffffffffu, mbar_wait<kCluster>(bar, parity, abort, err));
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, err));
 }
 
 /* 2-D TMA tile load into shared memory, completing `bytes` on `bar`. (x, y): innermost coordinate
